@@ -492,6 +492,99 @@ int mvf_xty(
     const float *x, int32_t ldx, int32_t A, const float *y, int32_t ldy, int32_t B, int64_t rows,
     float *out, int32_t ldo, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------------- *
+ * Rows kept in 8 bits for a backward pass (no counterpart in the reference,
+ * whose training keeps float32 activations; see its own note of 2.7 kB per
+ * pixel, conf/models/segmentation/multimodal/sparseconv3d.yaml:7270).
+ *
+ * Layout: codes int8 [rows][C]; exps uint8 [rows][ceil(C / 32)], one exponent
+ * byte e per 32 neighbouring columns of a row.  A value reads back as
+ * code * 2^(e - 133); e is the smallest with amax <= 127.5 * 2^(e - 133) for the
+ * group's largest finite magnitude (at most 254; 142 for float16 rows), codes
+ * are rounded to nearest, ties to even, within [-127, 127], so a finite value
+ * is off by at most half a step, 2^(e - 134) <= amax / 127.5 (one step at the
+ * very top of the type's range).  The code -128 stands for a value that is not
+ * finite and reads back as NaN; such a value leaves the rest of its group alone.
+ * type of rows: 0 float32, 1 bfloat16, 2 float16.
+ * ---------------------------------------------------------------------- */
+int mvf_pack_rows8(
+    const void *x, int32_t type, int64_t rows, int32_t C, int8_t *codes, uint8_t *exps, void *stream);
+int mvf_unpack_rows8(
+    const int8_t *codes, const uint8_t *exps, int64_t rows, int32_t C, void *y, int32_t type, void *stream);
+
+/* mvf_batch_norm_act_forward / _backward with the normalised input
+ * zhat = (z - mean) * invstd kept as 8-bit rows for the backward instead of z.
+ * forward: y [rows][C] (bit for bit the value of mvf_batch_norm_act_forward; may
+ * be NULL), codes / exps of zhat (computed in float64), save_invstd [C].  With an
+ * activation a code reads back on the side of the kink -beta / gamma (rounded
+ * to float32) on which the value lies: it is moved by at most one step for that.
+ * backward: the formulas of mvf_batch_norm_act_backward with zhat as read back
+ * and the activation's side taken from it; grad_z, grad_weight, grad_bias may be
+ * NULL.  weight and bias are the ones of the forward.  workspace:
+ * mvf_batch_norm_act8_workspace_bytes(C) bytes in both directions. */
+size_t mvf_batch_norm_act8_workspace_bytes(int32_t C);
+int mvf_batch_norm_act8_forward(
+    const float *z, int64_t rows, int32_t C, const float *weight, const float *bias,
+    float *running_mean, float *running_var, int32_t training, float momentum, float eps,
+    int32_t act, float slope, float *y, int8_t *codes, uint8_t *exps, float *save_invstd,
+    const double *col_sums, int32_t n_col_sums, void *workspace, size_t workspace_bytes, void *stream);
+int mvf_batch_norm_act8_backward(
+    const float *grad_y, const int8_t *codes, const uint8_t *exps, int64_t rows, int32_t C,
+    const float *weight, const float *bias, const float *save_invstd, int32_t training, int32_t act, float slope,
+    float *grad_z, float *grad_weight, float *grad_bias,
+    void *workspace, size_t workspace_bytes, void *stream);
+
+/* mvf_xty with the second operand as 8-bit rows: out[a][b] = sum over r of
+ * x[r][a] * y[r][b], the weight gradient of a Linear whose input was kept packed.
+ * tail == 0: y is the value read back.  tail != 0: the rows are the codes of
+ * mvf_batch_norm_act8_forward and y = act(bn_weight * zhat + bn_bias) (NULL: 1
+ * and 0; act, slope as there), i.e. the Linear behind that activation.
+ * x_sums (may be NULL): [A] the column sums of x, the bias gradient.  codes and
+ * exps are contiguous rows of B columns.  bf16 matrix cores, float32 operands cut
+ * exactly into bf16 parts, float32 accumulators, partial sums folded in a fixed
+ * order (the same bits on every run).  workspace: mvf_xty8_workspace_bytes(). */
+size_t mvf_xty8_workspace_bytes(void);
+int mvf_xty8(
+    const float *x, int32_t ldx, int32_t A, const int8_t *codes, const uint8_t *exps, int32_t B, int64_t rows,
+    int32_t tail, const float *bn_weight, const float *bn_bias, int32_t act, float slope,
+    float *out, int32_t ldo, float *x_sums, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------- *
+ * Gated residual block between two norms, e.g. a pooled image feature f onto the
+ * point's own feature x (the residual fusion behind the pools, with a gate per
+ * channel group as Gating makes it, modules/multimodal/pooling.py:702-723):
+ *   out = x + scale * gate * N(f; post),   h = N(out; pre)
+ * x, f, out, h: contiguous rows [rows][C], 1 <= C <= 4096, of `type` (0 float32,
+ * 1 bfloat16, 2 float16); f may be NULL (out = x).  post, pre: 0 none (N(v) = v; no
+ * h for pre), 1 RMS norm, 2 layer norm, with weight and bias [C] (NULL: 1 and 0).
+ * gate [rows][G] (NULL: 1): channel c takes gate[r][c / (C / G)], C % G == 0.
+ * scale [C] (NULL: 1).  seen [rows] (NULL: all): a row with seen == 0 adds
+ * nothing and its f is not read.  float32 arithmetic; out and h are rounded
+ * once each.  out may be NULL when pre is not 0.
+ * For a backward pass: stats [4][rows] float32 (1 / spread and mean of f and of
+ * out; NULL: not kept), and x_codes / x_exps, f_codes / f_exps: x and f as
+ * 8-bit rows (NULL: not kept).
+ * backward: d_out, d_h (either may be NULL: zero); x and f as they are, or as
+ * 8-bit rows with the pointers of the rows NULL; stats of the forward.  Outputs
+ * (each may be NULL): d_x, d_f rows; d_gate [rows][G]; d_scale, d_w_post,
+ * d_b_post, d_w_pre, d_b_pre [C], for which workspace holds
+ * mvf_residual_norm_workspace_bytes(rows, C) bytes.  Sums over rows are folded in
+ * a fixed order.
+ * ---------------------------------------------------------------------- */
+int mvf_residual_norm_forward(
+    const void *x, const void *f, int32_t type, int64_t rows, int32_t C, const float *gate, int32_t G,
+    const uint8_t *seen, const float *scale, int32_t post, const float *w_post, const float *b_post, float eps_post,
+    int32_t pre, const float *w_pre, const float *b_pre, float eps_pre, void *out, void *h,
+    int8_t *x_codes, uint8_t *x_exps, int8_t *f_codes, uint8_t *f_exps, float *stats, void *stream);
+size_t mvf_residual_norm_workspace_bytes(int64_t rows, int32_t C);
+int mvf_residual_norm_backward(
+    const void *d_out, const void *d_h, const void *x, const int8_t *x_codes, const uint8_t *x_exps,
+    const void *f, const int8_t *f_codes, const uint8_t *f_exps, int32_t type, int64_t rows, int32_t C,
+    const float *gate, int32_t G, const uint8_t *seen, const float *scale, int32_t post, const float *w_post,
+    const float *b_post, int32_t pre, const float *w_pre, const float *stats, void *d_x, void *d_f, float *d_gate,
+    float *d_scale, float *d_w_post, float *d_b_post, float *d_w_pre, float *d_b_pre,
+    void *workspace, size_t workspace_bytes, void *stream);
+
 /* Attention-weighted segment sum with a graph (pooling.py:289-296, 519-526:
  * segment_csr(x_mod * expand_group_feat(A), csr_idx, 'sum')) and its gradients.
  * out[s][c] = sum over the rows r of segment s of x[r][c] * att[r][g(c)], with G

@@ -14,12 +14,14 @@
 // float64 per thread, reduced per block in a fixed order and written as one partial row
 // per block; a second small kernel folds the partials in a fixed order, so the
 // statistics are the same on every run.
-#include "mvf_common.h"
+#include "mvf_bn_kink.h"
+#include "mvf_rows8.h"
 
 namespace mvf {
 
 constexpr int BN_THREADS = 256;
 constexpr int BN_MAX_BLOCKS = 1024;
+constexpr int BN8_MAX_BLOCKS = 4096;
 constexpr int BN_FOLD_COLS = 4;         // columns per block of the fold kernels
 
 template <int VW> __device__ __forceinline__ void bn_load(const float *p, float (&v)[VW])
@@ -245,7 +247,7 @@ __device__ __forceinline__ void bn_fold(const double *partial, int nblk, int C, 
 __global__ __launch_bounds__(BN_THREADS) void bn_stats_kernel(
     const double *__restrict__ partial, int nblk, int C, i64 rows, float eps, float momentum,
     float *__restrict__ running_mean, float *__restrict__ running_var,
-    float *__restrict__ save_mean, float *__restrict__ save_invstd)
+    float *__restrict__ save_mean, float *__restrict__ save_invstd, double *__restrict__ terms64)
 {
     double S, Q;
     bool owner;
@@ -257,7 +259,12 @@ __global__ __launch_bounds__(BN_THREADS) void bn_stats_kernel(
     double var = Q / n - mean * mean;
     if (var < 0.0) var = 0.0;
     save_mean[col] = (float)mean;
-    save_invstd[col] = (float)(1.0 / sqrt(var + (double)eps));
+    const double invstd = 1.0 / sqrt(var + (double)eps);
+    save_invstd[col] = (float)invstd;
+    if (terms64) {
+        terms64[col] = mean;
+        terms64[C + col] = invstd;
+    }
     if (running_mean) running_mean[col] = (float)((1.0 - (double)momentum) * (double)running_mean[col] + (double)momentum * mean);
     if (running_var) {
         const double unbiased = rows > 1 ? var * n / (n - 1.0) : var;
@@ -268,12 +275,17 @@ __global__ __launch_bounds__(BN_THREADS) void bn_stats_kernel(
 // Normalisation terms from the running statistics (eval mode with a graph).
 __global__ void bn_running_terms_kernel(
     const float *__restrict__ running_mean, const float *__restrict__ running_var, int C, float eps,
-    float *__restrict__ save_mean, float *__restrict__ save_invstd)
+    float *__restrict__ save_mean, float *__restrict__ save_invstd, double *__restrict__ terms64)
 {
     const int c = blockIdx.x * blockDim.x + threadIdx.x;
     if (c >= C) return;
     save_mean[c] = running_mean[c];
-    save_invstd[c] = (float)(1.0 / sqrt((double)running_var[c] + (double)eps));
+    const double invstd = 1.0 / sqrt((double)running_var[c] + (double)eps);
+    save_invstd[c] = (float)invstd;
+    if (terms64) {
+        terms64[c] = (double)running_mean[c];
+        terms64[C + c] = invstd;
+    }
 }
 
 // Gradients of weight and bias, and the two per-column means the input gradient needs.
@@ -386,6 +398,196 @@ __global__ __launch_bounds__(BN_THREADS) void bn_grad_apply_kernel(
     }
 }
 
+// ---- the same tail with its normalised input kept in 8 bits ---------------------------------------
+// What the backward reads is the 8-bit form (mvf_rows8.h) of zhat = (z - mean) * invstd instead of z:
+// a byte per value, and 9 instead of 12 bytes per value in the pass that writes grad_z.  zhat and its
+// code are computed in float64 (a few of the vector unit's idle cycles in a pass bound by HBM), so
+// that a code does not depend on how the statistics were rounded.  (BnKink: mvf_bn_kink.h keeps a
+// code on its own side of the activation's kink.)
+
+// y = act((z - mean) * invstd * gamma + beta) (bn_apply_kernel's value; y may be NULL) and the codes
+// of zhat.
+template <bool VEC>
+__global__ __launch_bounds__(BN_THREADS) void bn_apply8_kernel(
+    const float *__restrict__ z, i64 rows, int C, i64 rows_per_block,
+    const float *__restrict__ save_mean, const float *__restrict__ save_invstd, const double *__restrict__ terms64,
+    const float *__restrict__ weight, const float *__restrict__ bias, int act, float slope,
+    float *__restrict__ y, int8_t *__restrict__ codes, uint8_t *__restrict__ exps)
+{
+    const R8Walk w = r8_walk<true>(rows, C, rows_per_block);
+    const int G = (C + R8_GROUP - 1) / R8_GROUP;
+    const bool live = w.col < C, lead = (threadIdx.x & 7) == 0;
+    float mean[4], invstd[4], gamma[4], beta[4];
+    double mean64[4], invstd64[4];
+    BnKink kink[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int c = min(w.col + j, C - 1);
+        mean[j] = save_mean[c];
+        invstd[j] = save_invstd[c];
+        mean64[j] = terms64[c];
+        invstd64[j] = terms64[C + c];
+        gamma[j] = weight ? weight[c] : 1.0f;
+        beta[j] = bias ? bias[c] : 0.0f;
+        kink[j].load(gamma[j], beta[j]);
+    }
+    auto one = [&](i64 r, const float (&v)[4]) {
+        double zh[4];
+        unsigned m = 0;
+        float zf[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            zh[j] = ((double)v[j] - mean64[j]) * invstd64[j];
+            zf[j] = (float)zh[j];
+            if (VEC ? live : w.col + j < C) m = max(m, r8_magnitude(zf[j]));
+        }
+        const int e = r8_exponent(r8_max8(m), R8_E_MAX);
+        int q[4];
+        float o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float c = (float)rint(ldexp(zh[j], R8_BIAS - e));
+            if (act) c = kink[j].side(c, zh[j] * (double)gamma[j] + (double)beta[j] > 0.0, e);
+            c = fminf(fmaxf(c, -127.0f), 127.0f);
+            q[j] = (__float_as_uint(zf[j]) & 0x7f800000u) == 0x7f800000u ? R8_NAN : (int)c;
+            const float a = (v[j] - mean[j]) * invstd[j] * gamma[j] + beta[j];
+            o[j] = (act && !(a > 0.0f)) ? a * slope : a;
+        }
+        if (live) {
+            codes_store4<VEC>(codes + r * C, w.col, C, r8_pack4(q));
+            if (y) row_store4<RowF32, VEC>(y + r * C, w.col, C, o);
+        }
+        if (lead) exps[r * G + w.col / R8_GROUP] = (uint8_t)e;
+    };
+    i64 r = w.r0;
+    for (; r + 3 * (i64)w.rstep < w.rend; r += 4 * (i64)w.rstep) {
+        float v[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[u][j] = 0.0f;
+            if (live) row_load4<RowF32, VEC>(z + (r + (i64)u * w.rstep) * C, w.col, C, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) one(r + (i64)u * w.rstep, v[u]);
+    }
+    for (; r < w.rend; r += w.rstep) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (live) row_load4<RowF32, VEC>(z + r * C, w.col, C, v);
+        one(r, v);
+    }
+}
+
+// Column sums of g and g * zhat from the codes (bn_grad_sums_kernel's, with zhat as it is read back).
+template <int VW>
+__global__ __launch_bounds__(BN_THREADS) void bn_grad_sums8_kernel(
+    const float *__restrict__ gy, const int8_t *__restrict__ codes, const uint8_t *__restrict__ exps,
+    i64 rows, int C, i64 rows_per_block, const float *__restrict__ weight, const float *__restrict__ bias,
+    int act, float slope, double *__restrict__ partial)
+{
+    const BnWalk w = bn_walk<VW>(rows, C, rows_per_block);
+    const int G = (C + R8_GROUP - 1) / R8_GROUP;
+    double s[VW], q[VW];
+#pragma unroll
+    for (int j = 0; j < VW; ++j) s[j] = q[j] = 0.0;
+    if (w.col >= 0) {
+        BnKink kink[VW];
+#pragma unroll
+        for (int j = 0; j < VW; ++j) kink[j].load(weight ? weight[w.col + j] : 1.0f, bias ? bias[w.col + j] : 0.0f);
+        const int grp = w.col / R8_GROUP;
+        auto load = [&](i64 r, float (&g)[VW], unsigned &c, int &e) {
+            bn_load<VW>(gy + r * C + w.col, g);
+            if constexpr (VW == 4) c = *reinterpret_cast<const unsigned *>(codes + r * C + w.col);
+            else c = (unsigned)(uint8_t)codes[r * C + w.col];
+            e = exps[r * G + grp];
+        };
+        auto add = [&](const float (&g)[VW], unsigned c, int e) {
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const float zh = r8_decode(r8_byte(c, j), e);
+                const float gg = (act && !kink[j].on(zh)) ? g[j] * slope : g[j];
+                s[j] += (double)gg;
+                q[j] += (double)gg * (double)zh;
+            }
+        };
+        i64 r = w.r0;
+        for (; r + 3 * (i64)w.rstep < w.rend; r += 4 * (i64)w.rstep) {
+            float g[4][VW];
+            unsigned c[4];
+            int e[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load(r + (i64)u * w.rstep, g[u], c[u], e[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) add(g[u], c[u], e[u]);
+        }
+        for (; r < w.rend; r += w.rstep) {
+            float g[VW];
+            unsigned c;
+            int e;
+            load(r, g, c, e);
+            add(g, c, e);
+        }
+    }
+    bn_block_fold<VW>(s, q, C, partial);
+}
+
+// grad_z from the codes (bn_grad_apply_kernel's formula).
+template <int VW>
+__global__ __launch_bounds__(BN_THREADS) void bn_grad_apply8_kernel(
+    const float *__restrict__ gy, const int8_t *__restrict__ codes, const uint8_t *__restrict__ exps,
+    i64 rows, int C, i64 rows_per_block, const float *__restrict__ save_invstd,
+    const float *__restrict__ weight, const float *__restrict__ bias, int act, float slope,
+    const float *__restrict__ col_terms, int training, float *__restrict__ gz)
+{
+    const BnWalk w = bn_walk<VW>(rows, C, rows_per_block);
+    if (w.col < 0) return;
+    const int G = (C + R8_GROUP - 1) / R8_GROUP, grp = w.col / R8_GROUP;
+    float m_g[VW], m_gz[VW], k[VW];
+    BnKink kink[VW];
+#pragma unroll
+    for (int j = 0; j < VW; ++j) {
+        const float gamma = weight ? weight[w.col + j] : 1.0f;
+        kink[j].load(gamma, bias ? bias[w.col + j] : 0.0f);
+        m_g[j] = training ? col_terms[w.col + j] : 0.0f;
+        m_gz[j] = training ? col_terms[C + w.col + j] : 0.0f;
+        k[j] = gamma * save_invstd[w.col + j];
+    }
+    auto load = [&](i64 r, float (&g)[VW], unsigned &c, int &e) {
+        bn_load<VW>(gy + r * C + w.col, g);
+        if constexpr (VW == 4) c = *reinterpret_cast<const unsigned *>(codes + r * C + w.col);
+        else c = (unsigned)(uint8_t)codes[r * C + w.col];
+        e = exps[r * G + grp];
+    };
+    auto store = [&](i64 r, const float (&g)[VW], unsigned c, int e) {
+        float v[VW];
+#pragma unroll
+        for (int j = 0; j < VW; ++j) {
+            const float zh = r8_decode(r8_byte(c, j), e);
+            const float gg = (act && !kink[j].on(zh)) ? g[j] * slope : g[j];
+            // (running statistics: m_gz is zero, and a value that is not finite stays with its own row)
+            v[j] = training ? (gg - m_g[j] - zh * m_gz[j]) * k[j] : gg * k[j];
+        }
+        bn_store<VW>(gz + r * C + w.col, v);
+    };
+    i64 r = w.r0;
+    for (; r + 3 * (i64)w.rstep < w.rend; r += 4 * (i64)w.rstep) {
+        float g[4][VW];
+        unsigned c[4];
+        int e[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) load(r + (i64)u * w.rstep, g[u], c[u], e[u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) store(r + (i64)u * w.rstep, g[u], c[u], e[u]);
+    }
+    for (; r < w.rend; r += w.rstep) {
+        float g[VW];
+        unsigned c;
+        int e;
+        load(r, g, c, e);
+        store(r, g, c, e);
+    }
+}
+
 // Launch shape of the row-walking kernels: (row blocks, column chunks), rows per block a
 // multiple of the rows a block covers per pass.
 struct BnGrid {
@@ -456,10 +658,11 @@ extern "C" int mvf_batch_norm_act_forward(
         }
         hipLaunchKernelGGL(bn_stats_kernel, dim3(cdiv(C, BN_FOLD_COLS)), dim3(BN_THREADS), 0, st,
                            partial, nblk, C, (i64)rows, eps, momentum,
-                           running_mean, running_var, save_mean, save_invstd);
+                           running_mean, running_var, save_mean, save_invstd, (double *)nullptr);
     } else {
         hipLaunchKernelGGL(bn_running_terms_kernel, dim3(cdiv(C, 256)), dim3(256), 0, st,
-                           (const float *)running_mean, (const float *)running_var, C, eps, save_mean, save_invstd);
+                           (const float *)running_mean, (const float *)running_var, C, eps, save_mean, save_invstd,
+                           (double *)nullptr);
     }
     if (vec)
         hipLaunchKernelGGL(bn_apply_kernel<4>, g.grid, dim3(BN_THREADS), 0, st, z, (i64)rows, C, g.rows_per_block,
@@ -504,6 +707,99 @@ extern "C" int mvf_batch_norm_act_backward(
         hipLaunchKernelGGL(bn_grad_apply_kernel<1>, g.grid, dim3(BN_THREADS), 0, st, grad_y, z, (i64)rows, C,
                            g.rows_per_block, save_mean, save_invstd, weight, bias, act, slope,
                            (const float *)col_terms, training, grad_z);
+    MVF_LAUNCH_CHECK();
+    return MVF_OK;
+}
+
+extern "C" size_t mvf_batch_norm_act8_workspace_bytes(int32_t C)
+{
+    if (C < 1) return 0;
+    return mvf_batch_norm_act_workspace_bytes(C) + align_up(2 * (size_t)C * sizeof(double));
+}
+
+extern "C" int mvf_batch_norm_act8_forward(
+    const float *z, int64_t rows, int32_t C, const float *weight, const float *bias,
+    float *running_mean, float *running_var, int32_t training, float momentum, float eps,
+    int32_t act, float slope, float *y, int8_t *codes, uint8_t *exps, float *save_invstd,
+    const double *col_sums, int32_t n_col_sums, void *workspace, size_t workspace_bytes, void *stream)
+{
+    MVF_REQUIRE(rows >= 1 && C >= 1, "batch_norm_act8_forward: rows and C must be positive");
+    MVF_REQUIRE(z && codes && exps && save_invstd, "batch_norm_act8_forward: null argument");
+    MVF_REQUIRE(training || (running_mean && running_var),
+                "batch_norm_act8_forward: running statistics are needed outside train mode");
+    MVF_REQUIRE(!training || rows > 1, "batch_norm_act8_forward: more than one row per channel is needed in train mode");
+    MVF_REQUIRE(workspace && workspace_bytes >= mvf_batch_norm_act8_workspace_bytes(C),
+                "batch_norm_act8_forward: workspace too small");
+    MVF_REQUIRE(!col_sums || n_col_sums >= 1, "batch_norm_act8_forward: column sums without partial rows");
+    hipStream_t st = (hipStream_t)stream;
+    double *mine = (double *)workspace;
+    float *mean = (float *)((char *)workspace + bn_partial_bytes(C));
+    double *terms64 = (double *)((char *)workspace + mvf_batch_norm_act_workspace_bytes(C));
+    if (training) {
+        const double *partial = col_sums;
+        int nblk = n_col_sums;
+        if (!col_sums) {
+            const bool vec = C % 4 == 0 && (uintptr_t)z % 16 == 0;
+            const BnGrid g = bn_grid(rows, C, vec ? 4 : 1);
+            if (vec) hipLaunchKernelGGL(bn_sums_kernel<4>, g.grid, dim3(BN_THREADS), 0, st, z, (i64)rows, C, g.rows_per_block, mine);
+            else hipLaunchKernelGGL(bn_sums_kernel<1>, g.grid, dim3(BN_THREADS), 0, st, z, (i64)rows, C, g.rows_per_block, mine);
+            partial = mine;
+            nblk = g.nblk;
+        }
+        hipLaunchKernelGGL(bn_stats_kernel, dim3(cdiv(C, BN_FOLD_COLS)), dim3(BN_THREADS), 0, st,
+                           partial, nblk, C, (i64)rows, eps, momentum,
+                           running_mean, running_var, mean, save_invstd, terms64);
+    } else {
+        hipLaunchKernelGGL(bn_running_terms_kernel, dim3(cdiv(C, 256)), dim3(256), 0, st,
+                           (const float *)running_mean, (const float *)running_var, C, eps, mean, save_invstd, terms64);
+    }
+    const bool vec = C % 4 == 0 && (uintptr_t)z % 16 == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)codes % 4 == 0;
+    const R8Grid g = r8_grid(rows, C, true, 4, BN8_MAX_BLOCKS);
+    if (vec)
+        hipLaunchKernelGGL(bn_apply8_kernel<true>, g.grid, dim3(BN_THREADS), 0, st, z, (i64)rows, C, g.rows_per_block,
+                           (const float *)mean, (const float *)save_invstd, (const double *)terms64, weight, bias,
+                           act, slope, y, codes, exps);
+    else
+        hipLaunchKernelGGL(bn_apply8_kernel<false>, g.grid, dim3(BN_THREADS), 0, st, z, (i64)rows, C, g.rows_per_block,
+                           (const float *)mean, (const float *)save_invstd, (const double *)terms64, weight, bias,
+                           act, slope, y, codes, exps);
+    MVF_LAUNCH_CHECK();
+    return MVF_OK;
+}
+
+extern "C" int mvf_batch_norm_act8_backward(
+    const float *grad_y, const int8_t *codes, const uint8_t *exps, int64_t rows, int32_t C,
+    const float *weight, const float *bias, const float *save_invstd, int32_t training, int32_t act, float slope,
+    float *grad_z, float *grad_weight, float *grad_bias,
+    void *workspace, size_t workspace_bytes, void *stream)
+{
+    MVF_REQUIRE(rows >= 1 && C >= 1, "batch_norm_act8_backward: rows and C must be positive");
+    MVF_REQUIRE(grad_y && codes && exps && save_invstd, "batch_norm_act8_backward: null argument");
+    MVF_REQUIRE(workspace && workspace_bytes >= mvf_batch_norm_act8_workspace_bytes(C),
+                "batch_norm_act8_backward: workspace too small");
+    hipStream_t st = (hipStream_t)stream;
+    const bool vec = C % 4 == 0 && (uintptr_t)grad_y % 16 == 0 && (uintptr_t)grad_z % 16 == 0 && (uintptr_t)codes % 4 == 0;
+    const BnGrid g = bn_grid(rows, C, vec ? 4 : 1);
+    double *partial = (double *)workspace;
+    float *col_terms = (float *)((char *)workspace + bn_partial_bytes(C));
+    if ((training && grad_z) || grad_weight || grad_bias) {
+        if (vec)
+            hipLaunchKernelGGL(bn_grad_sums8_kernel<4>, g.grid, dim3(BN_THREADS), 0, st, grad_y, codes, exps, (i64)rows, C,
+                               g.rows_per_block, weight, bias, act, slope, partial);
+        else
+            hipLaunchKernelGGL(bn_grad_sums8_kernel<1>, g.grid, dim3(BN_THREADS), 0, st, grad_y, codes, exps, (i64)rows, C,
+                               g.rows_per_block, weight, bias, act, slope, partial);
+        hipLaunchKernelGGL(bn_grad_terms_kernel, dim3(cdiv(C, BN_FOLD_COLS)), dim3(BN_THREADS), 0, st,
+                           (const double *)partial, g.nblk, C, (i64)rows, grad_weight, grad_bias, col_terms);
+    }
+    if (grad_z) {
+        if (vec)
+            hipLaunchKernelGGL(bn_grad_apply8_kernel<4>, g.grid, dim3(BN_THREADS), 0, st, grad_y, codes, exps, (i64)rows, C,
+                               g.rows_per_block, save_invstd, weight, bias, act, slope, (const float *)col_terms, training, grad_z);
+        else
+            hipLaunchKernelGGL(bn_grad_apply8_kernel<1>, g.grid, dim3(BN_THREADS), 0, st, grad_y, codes, exps, (i64)rows, C,
+                               g.rows_per_block, save_invstd, weight, bias, act, slope, (const float *)col_terms, training, grad_z);
+    }
     MVF_LAUNCH_CHECK();
     return MVF_OK;
 }

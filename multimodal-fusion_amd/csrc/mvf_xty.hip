@@ -14,7 +14,8 @@
 // every workgroup writes one partial result and a second kernel adds the partials in workgroup
 // order: no atomics, the same bits on every run.  The pass is bound by HBM (4 (A + B) bytes per
 // row).
-#include "mvf_common.h"
+#include "mvf_bn_kink.h"
+#include "mvf_rows8.h"
 
 namespace mvf {
 
@@ -248,6 +249,298 @@ __global__ __launch_bounds__(XTY_FOLD_SLOTS * XTY_FOLD_SLICES) void xty_fold_ker
     if (a < A && b < B) out[(size_t)a * ldo + b] = (float)s;
 }
 
+// ---- the same reduction with the second operand kept in 8 bits -------------------------------------
+// out[a][b] = sum over r of x[r][a] * y[r][b], y read from its 8-bit form (mvf_rows8.h): the weight
+// gradient of a Linear whose input was kept as packed rows (RAW), or of a Linear behind BatchNorm +
+// LeakyReLU of which only the packed normalised rows were kept (TAIL: y = act(gamma * zq + beta),
+// recomputed here, so that neither the activated rows nor the Linear's input exist in the backward).
+//
+// bf16 matrix cores (v_mfma_f32_32x32x16_bf16, 16 times the rate of the float32 form).  A value read
+// back has 7 significant bits and a power of two: one bf16 holds it exactly.  A float32 x is cut
+// into three bf16 parts by truncation (8 + 8 + 8 bits, exact), so RAW is three products per block,
+// each exact, accumulated in float32; TAIL cuts y into three parts as well and takes the six
+// products above 2^-24 of the result.  (A magnitude that is not finite in x, or NaN in y, makes
+// the sums it enters NaN.)
+//
+// Operands come straight from global memory: lane (n, kh) owns columns of a block and the 8 rows
+// 8 kh .. 8 kh + 7 of a step of 16, 128 to 256 contiguous bytes per row and load.  Steps are dealt to
+// the waves in turn; one step is in flight while the one before is cut and multiplied.
+typedef __bf16 xty_bf8 __attribute__((ext_vector_type(8)));
+typedef unsigned xty_u4 __attribute__((ext_vector_type(4)));
+
+constexpr int XTY8_STEP = 16;
+constexpr int XTY8_WGS = 2;          // workgroups per compute unit
+
+__device__ __forceinline__ xty_acc xty_mfma16(xty_u4 a, xty_u4 b, xty_acc c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(xty_bf8, a), __builtin_bit_cast(xty_bf8, b), c, 0, 0, 0);
+}
+
+// high halves of two floats as two bf16 (the first in the low half)
+__device__ __forceinline__ unsigned xty_hi2(float a, float b)
+{
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+
+// 8 float32 as bf16 parts: v = p[0] + p[1] + p[2] exactly for PARTS == 3, p[0] alone for values that
+// one bf16 holds
+template <int PARTS> struct XtyParts {
+    xty_u4 p[PARTS];
+    __device__ __forceinline__ void cut(const float (&v)[8])
+    {
+        float r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = v[j];
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) p[k][h] = xty_hi2(r[2 * h], r[2 * h + 1]);
+            if (k + 1 < PARTS)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[j] -= __uint_as_float(__float_as_uint(r[j]) & 0xffff0000u);
+        }
+    }
+};
+
+struct XtyTail {            // TAIL: the column terms of y = act(gamma * zq + beta)
+    const float *weight, *bias;     // may be NULL (1 and 0)
+    int act;
+    float slope;
+};
+
+template <int NA, int NB, bool TAIL, bool VX, bool VQ>
+__global__ __launch_bounds__(XTY_THREADS) void xty8_kernel(
+    const float *__restrict__ x, int ldx, int A, const int8_t *__restrict__ codes, int ldq, int B,
+    const uint8_t *__restrict__ exps, int lde, i64 rows, XtyTail tail, int want_sums,
+    float *__restrict__ partial, float *__restrict__ partial_sums)
+{
+    static_assert((!VX || NA == 2) && (!VQ || NB == 2), "operand forms");
+    __shared__ float fold[NA * NB * 16 * 64];
+    __shared__ float fold_sums[XTY_WAVES][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, kh = lane >> 5;
+    // columns of the lane in each block (past the width: column 0, never stored)
+    int xc[NA], qc[NB];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+        const int c = VX ? 2 * n + i : 32 * i + n;
+        xc[i] = c < A ? c : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int c = VQ ? 2 * n + i : 32 * i + n;
+        qc[i] = c < B ? c : 0;
+    }
+    float gamma[NB], beta[NB];
+    BnKink kink[NB];
+    if constexpr (TAIL) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            gamma[i] = tail.weight ? tail.weight[qc[i]] : 1.0f;
+            beta[i] = tail.bias ? tail.bias[qc[i]] : 0.0f;
+            kink[i].load(gamma[i], beta[i]);
+        }
+    }
+    xty_acc acc[NA][NB];
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    float sums[NA];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) sums[i] = 0.0f;
+
+    struct Step {
+        float x[NA][8];
+        int q[NB][8];
+        int e[VQ ? 1 : NB][8];
+    };
+    // live: rows of the step that exist (a row past the end counts as zeros and reads the last row)
+    auto load = [&](Step &s, i64 base, int live) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = 8 * kh + j;
+            const i64 r = base + (k < live ? k : live - 1);
+            const float *xr = x + r * ldx;
+            const int8_t *qr = codes + r * ldq;
+            const uint8_t *er = exps + r * lde;
+            if constexpr (VX) {
+                const xty_f2 t = *(const xty_f2 *)(xr + xc[0]);
+                s.x[0][j] = t.x;
+                s.x[1][j] = t.y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < NA; ++i) s.x[i][j] = xr[xc[i]];
+            }
+            if constexpr (VQ) {
+                const int t = *(const short *)(qr + qc[0]);
+                s.q[0][j] = (int)(t << 24) >> 24;
+                s.q[1][j] = t >> 8;
+                s.e[0][j] = er[qc[0] / R8_GROUP];
+            } else {
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    s.q[i][j] = qr[qc[i]];
+                    s.e[i][j] = er[qc[i] / R8_GROUP];
+                }
+            }
+        }
+    };
+    auto multiply = [&](Step &s, int live) {
+        if (live < XTY8_STEP) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool ok = 8 * kh + j < live;
+#pragma unroll
+                for (int i = 0; i < NA; ++i) s.x[i][j] = ok ? s.x[i][j] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) s.q[i][j] = ok ? s.q[i][j] : 0;
+            }
+        }
+        XtyParts<3> xp[NA];
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            xp[i].cut(s.x[i]);
+            if (want_sums)
+                sums[i] += ((s.x[i][0] + s.x[i][1]) + (s.x[i][2] + s.x[i][3])) + ((s.x[i][4] + s.x[i][5]) + (s.x[i][6] + s.x[i][7]));
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = r8_decode(s.q[j][k], s.e[VQ ? 0 : j][k]);
+                if constexpr (TAIL) {
+                    const float a = __fmaf_rn(v[k], gamma[j], beta[j]);
+                    v[k] = (tail.act && !kink[j].on(v[k])) ? a * tail.slope : a;
+                }
+            }
+            XtyParts<TAIL ? 3 : 1> yp;
+            yp.cut(v);
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                if constexpr (TAIL) {
+                    acc[i][j] = xty_mfma16(xp[i].p[2], yp.p[0], acc[i][j]);
+                    acc[i][j] = xty_mfma16(xp[i].p[1], yp.p[1], acc[i][j]);
+                    acc[i][j] = xty_mfma16(xp[i].p[0], yp.p[2], acc[i][j]);
+                    acc[i][j] = xty_mfma16(xp[i].p[1], yp.p[0], acc[i][j]);
+                    acc[i][j] = xty_mfma16(xp[i].p[0], yp.p[1], acc[i][j]);
+                    acc[i][j] = xty_mfma16(xp[i].p[0], yp.p[0], acc[i][j]);
+                } else {
+                    acc[i][j] = xty_mfma16(xp[i].p[2], yp.p[0], acc[i][j]);
+                    acc[i][j] = xty_mfma16(xp[i].p[1], yp.p[0], acc[i][j]);
+                    acc[i][j] = xty_mfma16(xp[i].p[0], yp.p[0], acc[i][j]);
+                }
+            }
+        }
+    };
+
+    const i64 nstep = rows / XTY8_STEP;         // whole steps
+    const i64 nwaves = (i64)gridDim.x * XTY_WAVES;
+    i64 b = (i64)blockIdx.x * XTY_WAVES + wave;
+    const bool last = b == nstep % nwaves;      // the wave whose turn the rows behind them are
+    Step s0, s1;
+    if (b < nstep) {
+        load(s0, b * XTY8_STEP, XTY8_STEP);
+        b += nwaves;
+        for (; b + nwaves < nstep; b += 2 * nwaves) {
+            __builtin_amdgcn_sched_barrier(0);
+            load(s1, b * XTY8_STEP, XTY8_STEP);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(s0, XTY8_STEP);
+            __builtin_amdgcn_sched_barrier(0);
+            load(s0, (b + nwaves) * XTY8_STEP, XTY8_STEP);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(s1, XTY8_STEP);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (b < nstep) {
+            load(s1, b * XTY8_STEP, XTY8_STEP);
+            multiply(s0, XTY8_STEP);
+            multiply(s1, XTY8_STEP);
+        } else {
+            multiply(s0, XTY8_STEP);
+        }
+    }
+    const int rest = (int)(rows - nstep * XTY8_STEP);
+    if (last && rest > 0) {
+        load(s0, nstep * XTY8_STEP, rest);
+        multiply(s0, rest);
+    }
+
+    // fold of the workgroup's waves, in wave order
+    for (int turn = 0; turn < XTY_WAVES; ++turn) {
+        if (wave == turn) {
+#pragma unroll
+            for (int i = 0; i < NA; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int at = ((i * NB + j) * 16 + e) * 64 + lane;
+                        fold[at] = turn == 0 ? acc[i][j][e] : fold[at] + acc[i][j][e];
+                    }
+        }
+        __syncthreads();
+    }
+    float *p = partial + (size_t)blockIdx.x * (NA * NB * 16 * 64);
+    for (int at = threadIdx.x; at < NA * NB * 16 * 64; at += XTY_THREADS) p[at] = fold[at];
+    if (want_sums) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const float t = sums[i] + __shfl_xor(sums[i], 32, 64);
+            if (kh == 0) fold_sums[wave][VX ? 2 * n + i : 32 * i + n] = t;
+        }
+        __syncthreads();
+        if (threadIdx.x < 32 * NA) {
+            float t = 0.0f;
+#pragma unroll
+            for (int k = 0; k < XTY_WAVES; ++k) t += fold_sums[k][threadIdx.x];
+            partial_sums[(size_t)blockIdx.x * 64 + threadIdx.x] = t;
+        }
+    }
+}
+
+// xty_fold_kernel, and in the blocks behind it the column sums of x: 16 columns a block.
+__global__ __launch_bounds__(XTY_FOLD_SLOTS * XTY_FOLD_SLICES) void xty8_fold_kernel(
+    const float *__restrict__ partial, const float *__restrict__ partial_sums, int nwg, int NA, int NB, int vx, int vy,
+    int A, int B, float *__restrict__ out, int ldo, float *__restrict__ sums)
+{
+    __shared__ double red[XTY_FOLD_SLICES][XTY_FOLD_SLOTS];
+    const int slot = threadIdx.x % XTY_FOLD_SLOTS, slice = threadIdx.x / XTY_FOLD_SLOTS;
+    const int nslots = NA * NB * 16 * 64;
+    const int at = blockIdx.x * XTY_FOLD_SLOTS + slot;
+    const bool of_sums = at >= nslots;                  // (whole blocks: nslots is a multiple of 16)
+    const float *src = of_sums ? partial_sums + (at - nslots) : partial + at;
+    const size_t stride = of_sums ? 64 : nslots;
+    const int per = (nwg + XTY_FOLD_SLICES - 1) / XTY_FOLD_SLICES;
+    const int k1 = min(nwg, (slice + 1) * per);
+    double s = 0.0;
+    for (int k = slice * per; k < k1; ++k) s += (double)src[k * stride];
+    red[slice][slot] = s;
+    __syncthreads();
+    if (slice != 0) return;
+    for (int k = 1; k < XTY_FOLD_SLICES; ++k) s += red[k][slot];
+    if (of_sums) {
+        if (at - nslots < A) sums[at - nslots] = (float)s;
+        return;
+    }
+    const int lane = at & 63, e = (at >> 6) & 15, blk = at >> 10;
+    const int m = (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5), n = lane & 31;
+    const int a = vx ? 2 * m + blk / NB : (blk / NB) * 32 + m;
+    const int b = vy ? 2 * n + blk % NB : (blk % NB) * 32 + n;
+    if (a < A && b < B) out[(size_t)a * ldo + b] = (float)s;
+}
+
+__global__ void xty8_zero_kernel(float *out, int A, int B, int ldo, float *sums)
+{
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < A * B) out[(size_t)(i / B) * ldo + i % B] = 0.0f;
+    if (sums && i < A) sums[i] = 0.0f;
+}
+
 }  // namespace mvf
 
 using namespace mvf;
@@ -315,6 +608,74 @@ extern "C" int mvf_xty(
             hipLaunchKernelGGL(xty_fold_kernel, dim3(NA * NB * 1024 / XTY_FOLD_SLOTS), dim3(XTY_FOLD_SLOTS * XTY_FOLD_SLICES), 0, st,
                                (const float *)partial, (int)nwg, NA, NB, (int)vx, (int)vy, At, Bt,
                                out + (size_t)a0 * ldo + b0, (int)ldo);
+        }
+    MVF_LAUNCH_CHECK();
+    return MVF_OK;
+}
+
+extern "C" size_t mvf_xty8_workspace_bytes(void)
+{
+    return mvf_xty_workspace_bytes() + align_up((size_t)XTY_MAX_WGS * 64 * sizeof(float));
+}
+
+extern "C" int mvf_xty8(
+    const float *x, int32_t ldx, int32_t A, const int8_t *codes, const uint8_t *exps, int32_t B, int64_t rows,
+    int32_t tail, const float *bn_weight, const float *bn_bias, int32_t act, float slope,
+    float *out, int32_t ldo, float *x_sums, void *workspace, size_t workspace_bytes, void *stream)
+{
+    MVF_REQUIRE(A >= 1 && B >= 1 && rows >= 0, "xty8: A and B must be positive, rows non-negative");
+    MVF_REQUIRE((i64)A * B < (1ll << 31), "xty8: A * B too large");
+    MVF_REQUIRE(out && ldo >= B, "xty8: null output or ldo < B");
+    MVF_REQUIRE(rows == 0 || (x && ldx >= A && codes && exps), "xty8: null input or a row stride below the width");
+    MVF_REQUIRE(workspace && workspace_bytes >= mvf_xty8_workspace_bytes(), "xty8: workspace too small");
+    hipStream_t st = (hipStream_t)stream;
+    if (rows == 0) {
+        const i64 n = (i64)A * B;
+        hipLaunchKernelGGL(xty8_zero_kernel, dim3(cdiv(n, 256)), dim3(256), 0, st, out, (int)A, (int)B, (int)ldo, x_sums);
+        MVF_LAUNCH_CHECK();
+        return MVF_OK;
+    }
+    int dev = 0, cus = 256;
+    if (hipGetDevice(&dev) == hipSuccess) {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && n > 0) cus = n;
+    }
+    float *partial = (float *)workspace;
+    float *partial_sums = (float *)((char *)workspace + mvf_xty_workspace_bytes());
+    const int lde = r8_groups(B);
+    for (int a0 = 0; a0 < A; a0 += 64)
+        for (int b0 = 0; b0 < B; b0 += 64) {
+            const int At = A - a0 < 64 ? A - a0 : 64, Bt = B - b0 < 64 ? B - b0 : 64;
+            const int NA = At > 32 ? 2 : 1, NB = Bt > 32 ? 2 : 1;
+            i64 nwg = (rows + XTY_WAVES * 64 - 1) / (XTY_WAVES * 64);
+            const i64 cap = (i64)cus * XTY8_WGS;
+            if (nwg > cap) nwg = cap;
+            if (nwg > XTY_MAX_WGS) nwg = XTY_MAX_WGS;
+            const float *xt = x + a0;
+            const int8_t *qt = codes + b0;
+            const uint8_t *et = exps + b0 / R8_GROUP;
+            const bool vx = NA == 2 && At % 2 == 0 && ldx % 2 == 0 && (uintptr_t)xt % 8 == 0;
+            const bool vq = NB == 2 && Bt % 2 == 0 && B % 2 == 0 && (uintptr_t)qt % 2 == 0;
+            const XtyTail tt = {bn_weight ? bn_weight + b0 : nullptr, bn_bias ? bn_bias + b0 : nullptr, (int)act, slope};
+            const int want = x_sums && b0 == 0;
+#define MVF_XTY8_LAUNCH(NA_, NB_, T_, VX_, VQ_)                                                                     \
+    hipLaunchKernelGGL((xty8_kernel<NA_, NB_, T_, VX_, VQ_>), dim3((unsigned)nwg), dim3(XTY_THREADS), 0, st, xt, (int)ldx, \
+                       At, qt, (int)B, Bt, et, lde, (i64)rows, tt, want, partial, partial_sums)
+#define MVF_XTY8_T(NA_, NB_, VX_, VQ_)                                                                              \
+    do { if (tail) MVF_XTY8_LAUNCH(NA_, NB_, true, VX_, VQ_); else MVF_XTY8_LAUNCH(NA_, NB_, false, VX_, VQ_); } while (0)
+            if (NA == 1 && NB == 1) MVF_XTY8_T(1, 1, false, false);
+            else if (NA == 1) { if (vq) MVF_XTY8_T(1, 2, false, true); else MVF_XTY8_T(1, 2, false, false); }
+            else if (NB == 1) { if (vx) MVF_XTY8_T(2, 1, true, false); else MVF_XTY8_T(2, 1, false, false); }
+            else if (vx && vq) MVF_XTY8_T(2, 2, true, true);
+            else if (vx) MVF_XTY8_T(2, 2, true, false);
+            else if (vq) MVF_XTY8_T(2, 2, false, true);
+            else MVF_XTY8_T(2, 2, false, false);
+#undef MVF_XTY8_T
+#undef MVF_XTY8_LAUNCH
+            hipLaunchKernelGGL(xty8_fold_kernel, dim3(NA * NB * 1024 / XTY_FOLD_SLOTS + (want ? 64 / XTY_FOLD_SLOTS : 0)),
+                               dim3(XTY_FOLD_SLOTS * XTY_FOLD_SLICES), 0, st, (const float *)partial,
+                               (const float *)partial_sums, (int)nwg, NA, NB, (int)vx, (int)vq, At, Bt,
+                               out + (size_t)a0 * ldo + b0, (int)ldo, want ? x_sums + a0 : nullptr);
         }
     MVF_LAUNCH_CHECK();
     return MVF_OK;

@@ -110,6 +110,22 @@ _SIGNATURES = {
                                               _P, _P, _P, _P, _SZ, _P]),
     "mvf_xty_workspace_bytes": (_SZ, []),
     "mvf_xty": (C.c_int, [_P, _I32, _I32, _P, _I32, _I32, _I64, _P, _I32, _P, _SZ, _P]),
+    "mvf_pack_rows8": (C.c_int, [_P, _I32, _I64, _I32, _P, _P, _P]),
+    "mvf_unpack_rows8": (C.c_int, [_P, _P, _I64, _I32, _P, _I32, _P]),
+    "mvf_batch_norm_act8_workspace_bytes": (_SZ, [_I32]),
+    "mvf_batch_norm_act8_forward": (C.c_int, [_P, _I64, _I32, _P, _P, _P, _P, _I32, _F, _F, _I32, _F,
+                                              _P, _P, _P, _P, _P, _I32, _P, _SZ, _P]),
+    "mvf_batch_norm_act8_backward": (C.c_int, [_P, _P, _P, _I64, _I32, _P, _P, _P, _I32, _I32, _F,
+                                               _P, _P, _P, _P, _SZ, _P]),
+    "mvf_xty8_workspace_bytes": (_SZ, []),
+    "mvf_xty8": (C.c_int, [_P, _I32, _I32, _P, _P, _I32, _I64, _I32, _P, _P, _I32, _F,
+                           _P, _I32, _P, _P, _SZ, _P]),
+    "mvf_residual_norm_forward": (C.c_int, [_P, _P, _I32, _I64, _I32, _P, _I32, _P, _P, _I32, _P, _P, _F,
+                                            _I32, _P, _P, _F, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "mvf_residual_norm_workspace_bytes": (_SZ, [_I64, _I32]),
+    "mvf_residual_norm_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _P, _I32, _P, _P,
+                                             _I32, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                             _P, _SZ, _P]),
     "mvf_weighted_segment_sum": (C.c_int, [_P, _P, _I32, _I32, _P, _I64, _P, _P]),
     "mvf_weighted_segment_sum_backward": (C.c_int, [_P, _P, _P, _I32, _I32, _P, _I64, _I64, _P, _P, _P]),
     "mvf_linear_rows_supported": (C.c_int, [_I32, _I32]),

@@ -1,0 +1,177 @@
+"""Gated residual block between two norms: what a pooled image feature (or any
+branch's output) goes through on its way onto a point's own feature,
+
+    out = x + scale * gate * N(f; post),    h = N(out; pre)
+
+in one kernel forward and one (and a fold of the column gradients) backward.
+``h`` is the input of the next branch.  The gate is one value per row and channel
+group, as ``pooling.Gating`` makes it (modules/multimodal/pooling.py:702-723);
+rows without a view (``seen``) pass through.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import packed
+from . import training
+
+_MAX_C = 4096
+_NONE, _RMS, _LAYER = 0, 1, 2
+
+
+def _norm_args(norm, C, x, name):
+    """(kind, weight, bias, eps) of an nn.RMSNorm / nn.LayerNorm over the channels."""
+    if norm is None:
+        return _NONE, None, None, 0.0
+    if isinstance(norm, torch.nn.LayerNorm):
+        kind = _LAYER
+    elif isinstance(norm, torch.nn.RMSNorm):
+        kind = _RMS
+    else:
+        raise TypeError(f"residual_norm: {name} must be an nn.RMSNorm or nn.LayerNorm, got {type(norm).__name__}")
+    if tuple(norm.normalized_shape) != (C,):
+        raise ValueError(f"residual_norm: {name} normalises {tuple(norm.normalized_shape)}, the rows have {C} channels")
+    eps = torch.finfo(x.dtype).eps if norm.eps is None else float(norm.eps)
+    return kind, _vector(norm.weight, C, x, name), _vector(getattr(norm, "bias", None), C, x, name), eps
+
+
+def _vector(t, C, x, name):
+    if t is None:
+        return None
+    if t.device != x.device:
+        raise ValueError(f"residual_norm: {name} is on {t.device}, the rows are on {x.device}")
+    if not t.is_floating_point() or t.numel() not in (1, C):
+        raise ValueError(f"residual_norm: {name} must hold 1 or {C} floating-point values, got {tuple(t.shape)} {t.dtype}")
+    return t.float().reshape(-1).expand(C)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """The kernels mvf_residual_norm_forward / _backward.  Kept for the backward:
+    x (only with a pre-norm) and f as they are or as 8-bit rows, four statistics a
+    row, and the parameters."""
+
+    @staticmethod
+    def forward(ctx, x, f, gate, scale, w_post, b_post, w_pre, b_pre, seen, post, pre, eps_post, eps_pre, keep):
+        lib = L.load()
+        x, f, gate, scale, w_post, b_post, w_pre, b_pre = (
+            None if t is None else t.detach().contiguous()
+            for t in (x, f, gate, scale, w_post, b_post, w_pre, b_pre))
+        rows, C = x.shape
+        dev = x.device
+        G = 0 if gate is None else gate.shape[1]
+        out = torch.empty_like(x)
+        h = torch.empty_like(x) if pre else None
+        wants = keep is not None
+        keep8 = keep == "int8"
+        xq = fq = (None, None)
+        if keep8:
+            def codes():
+                return (torch.empty((rows, C), dtype=torch.int8, device=dev),
+                        torch.empty((rows, packed._groups(C)), dtype=torch.uint8, device=dev))
+            xq = codes() if pre else xq
+            fq = codes() if f is not None else fq
+        stats = torch.empty((4, rows), dtype=torch.float32, device=dev) if wants and (pre or post) else None
+        with torch.cuda.device(dev):
+            L.check(lib.mvf_residual_norm_forward(
+                L.ptr(x), L.ptr(f), packed.ROW_TYPES[x.dtype], rows, C, L.ptr(gate), G, L.ptr(seen), L.ptr(scale),
+                post, L.ptr(w_post), L.ptr(b_post), eps_post, pre, L.ptr(w_pre), L.ptr(b_pre), eps_pre,
+                L.ptr(out), L.ptr(h), L.ptr(xq[0]), L.ptr(xq[1]), L.ptr(fq[0]), L.ptr(fq[1]), L.ptr(stats),
+                L.stream_ptr(dev)))
+        if wants:
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(
+                x if pre and not keep8 else None, xq[0], xq[1], None if keep8 else f, fq[0], fq[1],
+                gate, scale, w_post, b_post, w_pre, seen, stats)
+            ctx.args = rows, C, G, post, pre, x.dtype, dev
+        return (out, h) if pre else out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, d_h=None):
+        nothing = (None,) * 14
+        if d_out is None and d_h is None:
+            return nothing
+        lib = L.load()
+        x, xc, xe, f, fc, fe, gate, scale, w_post, b_post, w_pre, seen, stats = ctx.saved_tensors
+        rows, C, G, post, pre, dtype, dev = ctx.args
+        d_out = None if d_out is None else d_out.contiguous()
+        d_h = None if d_h is None else d_h.contiguous()
+        need = ctx.needs_input_grad
+
+        def empty(wanted, shape, kind=torch.float32):
+            return torch.empty(shape, dtype=kind, device=dev) if wanted else None
+
+        dx = empty(need[0], (rows, C), dtype)
+        df = empty(need[1], (rows, C), dtype)
+        dgate = empty(need[2], (rows, G))
+        vectors = [empty(need[i], (C,)) for i in range(3, 8)]
+        nbytes = lib.mvf_residual_norm_workspace_bytes(rows, C) if any(need[3:8]) else 0
+        ws = L.workspace(nbytes, dev) if nbytes else None
+        with torch.cuda.device(dev):
+            L.check(lib.mvf_residual_norm_backward(
+                L.ptr(d_out), L.ptr(d_h), L.ptr(x), L.ptr(xc), L.ptr(xe), L.ptr(f), L.ptr(fc), L.ptr(fe),
+                packed.ROW_TYPES[dtype], rows, C, L.ptr(gate), G, L.ptr(seen), L.ptr(scale),
+                post, L.ptr(w_post), L.ptr(b_post), pre, L.ptr(w_pre), L.ptr(stats), L.ptr(dx), L.ptr(df),
+                L.ptr(dgate), *(L.ptr(v) for v in vectors), L.ptr(ws), nbytes, L.stream_ptr(dev)))
+        return (dx, df, dgate, *vectors) + nothing[8:]
+
+
+def residual_norm(x, f, post=None, pre=None, gate=None, scale=None, seen=None, keep=None):
+    """``out = x + scale * gate * post(f)`` and, with ``pre``, ``h = pre(out)``:
+    returns ``out`` or ``(out, h)``, of the shape and type of x.
+
+    :param x: [..., C] float32, bfloat16 or float16 rows on the HIP device, C <= 4096
+    :param f: rows like x, the branch's output; None: out = x (the norm in front of
+        the first branch)
+    :param post, pre: nn.RMSNorm or nn.LayerNorm over the C channels, or None
+    :param gate: [...] or [..., G] with C % G == 0, G groups of neighbouring channels
+    :param scale: [C], one element, or a number
+    :param seen: [...] bool; where False nothing is added and f is not read, so
+        whatever it holds there (NaN included) reaches neither out nor a gradient
+    :param keep: what the backward keeps of x and f: 'float32' (the rows as they
+        are, whatever their type), 'int8' (``packed`` rows, gradients then come from
+        the values read back), or None: as ``training.keep_activations`` says
+
+    Arithmetic is float32, out and h are rounded once (h from the unrounded out).
+    Differentiable once with respect to x, f, gate, scale and the norms'
+    parameters."""
+    packed._check_rows(x, "residual_norm")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _MAX_C:
+        raise ValueError(f"residual_norm expects rows of 1 to {_MAX_C} channels, got {tuple(x.shape)}")
+    if f is None and not (post is None and gate is None and scale is None and seen is None):
+        raise ValueError("residual_norm: post, gate, scale and seen need f")
+    if f is None and pre is None:
+        raise ValueError("residual_norm: nothing to do without f and without pre")
+    shape, C = x.shape, x.shape[-1]
+    if f is not None and (f.shape != shape or f.dtype != x.dtype or f.device != x.device):
+        raise ValueError(f"residual_norm: f is {tuple(f.shape)} {f.dtype} on {f.device}, "
+                         f"x is {tuple(shape)} {x.dtype} on {x.device}")
+    k_post, w_post, b_post, eps_post = _norm_args(post, C, x, "post")
+    k_pre, w_pre, b_pre, eps_pre = _norm_args(pre, C, x, "pre")
+    rows = x.reshape(-1, C)
+    if gate is not None:
+        if gate.device != x.device or not gate.is_floating_point():
+            raise ValueError("residual_norm: gate must hold floating-point values on the device of the rows")
+        if gate.shape == shape[:-1]:
+            gate = gate.unsqueeze(-1)
+        if gate.shape[:-1] != shape[:-1] or gate.dim() != len(shape) or gate.shape[-1] < 1 or C % gate.shape[-1] != 0:
+            raise ValueError(f"residual_norm: gate {tuple(gate.shape)} does not fit rows {tuple(shape)}: one value per "
+                             f"row and channel group, in a number of groups that divides {C}")
+        gate = gate.float().reshape(-1, gate.shape[-1])
+    if scale is not None:
+        if not torch.is_tensor(scale):
+            scale = torch.full((C,), float(scale), dtype=torch.float32, device=x.device)
+        scale = _vector(scale, C, x, "scale")
+    if seen is not None:
+        if seen.dtype != torch.bool or seen.shape != shape[:-1] or seen.device != x.device:
+            raise ValueError(f"residual_norm: seen must be a bool tensor {tuple(shape[:-1])} on the device of the rows")
+        seen = seen.reshape(-1).contiguous().view(torch.uint8)
+    flat = None if f is None else f.reshape(-1, C)
+    leaves = (rows, flat, gate, scale, w_post, b_post, w_pre, b_pre)
+    keep = training.kept_form(keep)
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves)):
+        keep = None
+    got = _ResidualNorm.apply(*leaves, seen, k_post, k_pre, eps_post, eps_pre, keep)
+    if k_pre:
+        return got[0].view(shape), got[1].view(shape)
+    return got.view(shape)

@@ -13,19 +13,64 @@ BatchNorm1d + LeakyReLU tail one pair of this package's kernels forward and
 one backward (``batch_norm_act``), the attention-weighted sum one kernel each
 way (``weighted_segment_sum``), and the CSR operations are this package's
 kernels, all wrapped in ``torch.autograd.Function``
-(``pooling.segment_csr`` / ``gather_csr`` / ``segment_softmax_csr``).  The
-computation follows modules/multimodal/pooling.py: ``DeepSetFeat.forward``
+(``pooling.segment_csr`` / ``gather_csr`` / ``segment_softmax_csr``).
+
+Inside ``keep_activations('int8')`` (or with ``keep='int8'``) the dense layers keep
+8-bit rows (``packed``) for their backward instead of float32 ones: a Linear the
+rows it got, BatchNorm + LeakyReLU its normalised rows, and a Linear behind such
+an activation nothing of its own: its weight gradient is made of the packed
+rows of the activation.  The forward is the same bit for bit; gradients are the
+formulas' on the rows as they read back.
+
+The computation follows modules/multimodal/pooling.py: ``DeepSetFeat.forward``
 :658-681, ``MinMaxDiffSetFeat.forward`` :577-597, ``MLPSetFeat.forward``
 :688-699, ``GroupBimodalCSRPool.forward`` :263-315 and
 ``QKVBimodalCSRPool.forward`` :454-547.
 """
+import contextlib
 import ctypes
 import math
+import threading
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
+from . import packed
 from . import pooling as P
+
+_FORMS = ("float32", "int8")
+_kept = threading.local()
+
+
+@contextlib.contextmanager
+def keep_activations(form):
+    """Form in which the dense layers (and ``residual.residual_norm``) of this thread
+    keep rows for their backward pass: 'float32' (as they are, the default) or
+    'int8' (``packed`` rows).  Read by the forward; a backward uses what its forward
+    kept, wherever it runs."""
+    if form not in _FORMS:
+        raise ValueError(f"keep_activations: {form!r} is not one of {_FORMS}")
+    before = getattr(_kept, "form", _FORMS[0])
+    _kept.form = form
+    try:
+        yield
+    finally:
+        _kept.form = before
+
+
+def kept_form(keep=None):
+    """``keep``, or what ``keep_activations`` says where it is None."""
+    if keep is None:
+        return getattr(_kept, "form", _FORMS[0])
+    if keep not in _FORMS:
+        raise ValueError(f"keep={keep!r} is not one of {_FORMS}")
+    return keep
+
+
+def _keeps8(keep, *tensors):
+    return (kept_form(keep) == "int8" and torch.is_grad_enabled()
+            and any(t is not None and t.requires_grad for t in tensors))
 
 
 class _BatchNormAct(torch.autograd.Function):
@@ -78,19 +123,113 @@ class _BatchNormAct(torch.autograd.Function):
         return gz, gw, gb, None, None, None, None, None, None, None
 
 
-def batch_norm_act(z, bn, act, col_sums=None):
-    """``act(bn(z))`` for an ``nn.BatchNorm1d`` (train or eval mode, running
-    statistics and ``num_batches_tracked`` updated as the module does) followed
-    by a LeakyReLU, on this package's kernels when z is a float32 [rows, C]
-    tensor on the HIP device; other inputs and activations take the modules.
-    col_sums: partial column sums of z and z * z as ``linear(..., want_sums=True)``
-    returns them (batch statistics without another pass over z)."""
-    fused_act = isinstance(act, torch.nn.LeakyReLU)
+def _bn8_forward(z, weight, bias, rm, rv, eps, slope, batch_stats, factor, col_sums):
+    """(y, codes, exps, invstd) of mvf_batch_norm_act8_forward."""
+    lib = L.load()
+    rows, C = z.shape
+    dev = z.device
+    y = torch.empty_like(z)
+    codes = torch.empty((rows, C), dtype=torch.int8, device=dev)
+    exps = torch.empty((rows, packed._groups(C)), dtype=torch.uint8, device=dev)
+    invstd = torch.empty(C, dtype=torch.float32, device=dev)
+    nbytes = lib.mvf_batch_norm_act8_workspace_bytes(C)
+    ws = L.workspace(nbytes, dev)
+    with torch.cuda.device(dev):
+        L.check(lib.mvf_batch_norm_act8_forward(
+            L.ptr(z), rows, C, L.ptr(weight), L.ptr(bias), L.ptr(rm), L.ptr(rv), int(batch_stats),
+            float(factor), float(eps), int(slope is not None), 0.0 if slope is None else float(slope),
+            L.ptr(y), L.ptr(codes), L.ptr(exps), L.ptr(invstd),
+            L.ptr(col_sums), 0 if col_sums is None else col_sums.shape[0], L.ptr(ws), nbytes, L.stream_ptr(dev)))
+    return y, codes, exps, invstd
+
+
+def _bn8_backward(grad_y, codes, exps, weight, bias, invstd, batch_stats, slope, needs):
+    """(grad_z, grad_weight, grad_bias) of mvf_batch_norm_act8_backward, those of `needs`."""
+    lib = L.load()
+    rows, C = codes.shape
+    dev = codes.device
+    grad_y = grad_y.contiguous()
+    gz = torch.empty((rows, C), dtype=torch.float32, device=dev) if needs[0] else None
+    gw = torch.empty(C, dtype=torch.float32, device=dev) if needs[1] else None
+    gb = torch.empty(C, dtype=torch.float32, device=dev) if needs[2] else None
+    nbytes = lib.mvf_batch_norm_act8_workspace_bytes(C)
+    ws = L.workspace(nbytes, dev)
+    with torch.cuda.device(dev):
+        L.check(lib.mvf_batch_norm_act8_backward(
+            L.ptr(grad_y), L.ptr(codes), L.ptr(exps), rows, C, L.ptr(weight), L.ptr(bias), L.ptr(invstd),
+            int(batch_stats), int(slope is not None), 0.0 if slope is None else float(slope),
+            L.ptr(gz), L.ptr(gw), L.ptr(gb), L.ptr(ws), nbytes, L.stream_ptr(dev)))
+    return gz, gw, gb
+
+
+def _vector(t):
+    return None if t is None else t.detach().float().contiguous()
+
+
+class _BatchNormAct8(torch.autograd.Function):
+    """_BatchNormAct that keeps the normalised rows in 8 bits."""
+
+    @staticmethod
+    def forward(ctx, z, weight, bias, rm, rv, eps, slope, batch_stats, factor, col_sums):
+        w, b = _vector(weight), _vector(bias)
+        y, codes, exps, invstd = _bn8_forward(z.detach().contiguous(), w, b, rm, rv, eps, slope, batch_stats,
+                                              factor, col_sums)
+        ctx.save_for_backward(codes, exps, w, b, invstd)
+        ctx.slope, ctx.batch_stats = slope, bool(batch_stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        codes, exps, w, b, invstd = ctx.saved_tensors
+        return _bn8_backward(grad_y, codes, exps, w, b, invstd, ctx.batch_stats, ctx.slope,
+                             ctx.needs_input_grad) + (None,) * 7
+
+
+class _BatchNormActLinear8(torch.autograd.Function):
+    """Linear(act(bn(z))) that keeps the normalised rows in 8 bits and nothing else of
+    a row: the Linear's input is made of them again in its weight gradient."""
+
+    @staticmethod
+    def forward(ctx, z, bn_weight, bn_bias, weight, bias, rm, rv, eps, slope, batch_stats, factor, col_sums,
+                want_sums):
+        w, b = _vector(bn_weight), _vector(bn_bias)
+        y, codes, exps, invstd = _bn8_forward(z.detach().contiguous(), w, b, rm, rv, eps, slope, batch_stats,
+                                              factor, col_sums)
+        out, sums = _product(y, weight, bias, want_sums)
+        if sums is None:
+            sums = torch.empty(0, dtype=torch.float64, device=z.device)
+        ctx.save_for_backward(codes, exps, w, b, invstd, weight)
+        ctx.slope, ctx.batch_stats = slope, bool(batch_stats)
+        ctx.mark_non_differentiable(sums)
+        return out, sums
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, _grad_sums):
+        codes, exps, w, b, invstd, weight = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grad_out = grad_out.contiguous()
+        gz = gw = gb = glw = glb = None
+        if any(need[:3]):
+            gy = _product(grad_out, weight.t(), None)[0]
+            gz, gw, gb = _bn8_backward(gy, codes, exps, w, b, invstd, ctx.batch_stats, ctx.slope, need)
+        if need[3]:
+            glw, glb = xty8(grad_out, codes, exps, tail=(w, b, ctx.slope), want_sums=need[4])
+        elif need[4]:
+            glb = xty(grad_out).view(-1)
+        return (gz, gw, gb, glw, glb) + (None,) * 8
+
+
+def _bn_plan(z, bn):
+    """(running mean, running variance, batch_stats, factor) of an nn.BatchNorm1d's next
+    call on z, its num_batches_tracked counted; None where this package's kernels do not
+    take z or the module."""
     if not (z.is_cuda and z.dtype == torch.float32 and z.dim() == 2 and z.shape[0] > 0
             and isinstance(bn, torch.nn.BatchNorm1d)
             and all(t is None or (t.is_cuda and t.dtype == torch.float32)
                     for t in (bn.weight, bn.bias, bn.running_mean, bn.running_var))):
-        return act(bn(z))
+        return None
     batch_stats = bn.training or bn.running_mean is None
     factor = 0.0
     if batch_stats:
@@ -103,12 +242,45 @@ def batch_norm_act(z, bn, act, col_sums=None):
     # running statistics: updated in train mode, read in eval mode, unused by an eval-mode
     # module that tracks none (it normalises with batch statistics)
     use_running = bn.running_mean is not None and (bn.training or not batch_stats)
-    y = _BatchNormAct.apply(z, bn.weight, bn.bias,
-                            bn.running_mean if use_running else None,
-                            bn.running_var if use_running else None, bn.eps,
-                            float(act.negative_slope) if fused_act else None, batch_stats, factor,
-                            col_sums if batch_stats else None)
+    return (bn.running_mean if use_running else None, bn.running_var if use_running else None, batch_stats, factor)
+
+
+def batch_norm_act(z, bn, act, col_sums=None, keep=None):
+    """``act(bn(z))`` for an ``nn.BatchNorm1d`` (train or eval mode, running
+    statistics and ``num_batches_tracked`` updated as the module does) followed
+    by a LeakyReLU, on this package's kernels when z is a float32 [rows, C]
+    tensor on the HIP device; other inputs and activations take the modules.
+    col_sums: partial column sums of z and z * z as ``linear(..., want_sums=True)``
+    returns them (batch statistics without another pass over z).
+    keep: 'float32' keeps z for the backward, 'int8' its normalised rows in 8 bits
+    (a value that is not finite then counts as not above the activation's kink);
+    None: as ``keep_activations`` says."""
+    fused_act = isinstance(act, torch.nn.LeakyReLU)
+    keeps8 = _keeps8(keep, z, bn.weight, bn.bias)
+    plan = _bn_plan(z, bn)
+    if plan is None:
+        return act(bn(z))
+    rm, rv, batch_stats, factor = plan
+    fn = _BatchNormAct8 if keeps8 else _BatchNormAct
+    y = fn.apply(z, bn.weight, bn.bias, rm, rv, bn.eps, float(act.negative_slope) if fused_act else None,
+                 batch_stats, factor, col_sums if batch_stats else None)
     return y if fused_act else act(y)
+
+
+def batch_norm_act_linear(z, bn, act, lin, col_sums=None, want_sums=False, keep=None):
+    """``linear(lin, batch_norm_act(z, bn, act, col_sums), want_sums)``.  With 'int8'
+    rows (``keep``, ``keep_activations``) and a LeakyReLU the two keep one packed copy
+    of the normalised rows between them; elsewhere they are two calls."""
+    if (isinstance(act, torch.nn.LeakyReLU) and _takes(lin, z)
+            and _keeps8(keep, z, bn.weight, bn.bias, lin.weight, lin.bias)):
+        plan = _bn_plan(z, bn)
+        if plan is not None:
+            rm, rv, batch_stats, factor = plan
+            y, sums = _BatchNormActLinear8.apply(
+                z, bn.weight, bn.bias, lin.weight, lin.bias, rm, rv, bn.eps, float(act.negative_slope),
+                batch_stats, factor, col_sums if batch_stats else None, bool(want_sums))
+            return (y, sums if sums.numel() else None) if want_sums else y
+    return linear(lin, batch_norm_act(z, bn, act, col_sums=col_sums, keep=keep), want_sums, keep=keep)
 
 
 def xty(x, y=None):
@@ -203,31 +375,111 @@ class _Linear(torch.autograd.Function):
         return gx, gw, gb, None
 
 
-def linear(lin, x, want_sums=False):
+def xty8(x, codes, exps, tail=None, want_sums=False):
+    """(x^T . y, column sums of x or None) for float32 rows x and y read from 8-bit rows
+    (mvf_xty8).  tail = (weight, bias, slope): the rows are those of
+    ``mvf_batch_norm_act8_forward`` and y the activated values made of them."""
+    lib = L.load()
+    x = x.contiguous()
+    dev = x.device
+    A, B = x.shape[1], codes.shape[1]
+    out = torch.empty((A, B), dtype=torch.float32, device=dev)
+    sums = torch.empty(A, dtype=torch.float32, device=dev) if want_sums else None
+    w, b, slope = tail if tail is not None else (None, None, None)
+    nbytes = lib.mvf_xty8_workspace_bytes()
+    ws = L.workspace(nbytes, dev)
+    with torch.cuda.device(dev):
+        L.check(lib.mvf_xty8(
+            L.ptr(x), A, A, L.ptr(codes), L.ptr(exps), B, x.shape[0], int(tail is not None), L.ptr(w), L.ptr(b),
+            int(slope is not None), 0.0 if slope is None else float(slope), L.ptr(out), B, L.ptr(sums), L.ptr(ws),
+            nbytes, L.stream_ptr(dev)))
+    return out, sums
+
+
+class _Linear8(torch.autograd.Function):
+    """_Linear that keeps its input as 8-bit rows (nothing of it when the weight needs no
+    gradient)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, want_sums):
+        codes = exps = None
+        if ctx.needs_input_grad[1]:
+            codes, exps = packed.pack_codes(x.detach().contiguous())
+        ctx.save_for_backward(codes, exps, weight)
+        y, sums = _product(x, weight, bias, want_sums)
+        if sums is None:
+            sums = torch.empty(0, dtype=torch.float64, device=x.device)
+        ctx.mark_non_differentiable(sums)
+        return y, sums
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y, _grad_sums):
+        codes, exps, weight = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grad_y = grad_y.contiguous()
+        gx = _product(grad_y, weight.t(), None)[0] if need[0] else None
+        gw = gb = None
+        if need[1]:
+            gw, gb = xty8(grad_y, codes, exps, want_sums=need[2])
+        elif need[2]:
+            gb = xty(grad_y).view(-1)
+        return gx, gw, gb, None
+
+
+def _takes(lin, x):
+    return (x.is_cuda and x.dtype == torch.float32 and x.dim() == 2 and x.shape[0] > 0
+            and lin.weight.is_cuda and lin.weight.dtype == torch.float32)
+
+
+def _linear(x, weight, bias, want_sums=False, keep=None):
+    fn = _Linear8 if _keeps8(keep, x, weight, bias) else _Linear
+    return fn.apply(x, weight, bias, bool(want_sums))
+
+
+def linear(lin, x, want_sums=False, keep=None):
     """``lin(x)`` for an ``nn.Linear`` on float32 [rows, C] device tensors,
     with the weight gradient on this package's kernel; anything else takes the
     module.  want_sums: returns (output, partial column sums of the output and
-    its square or None) for ``batch_norm_act``."""
-    if (x.is_cuda and x.dtype == torch.float32 and x.dim() == 2 and x.shape[0] > 0
-            and lin.weight.is_cuda and lin.weight.dtype == torch.float32):
-        y, sums = _Linear.apply(x, lin.weight, lin.bias, bool(want_sums))
+    its square or None) for ``batch_norm_act``.  keep: 'float32' keeps x for the
+    weight gradient, 'int8' its 8-bit rows; None: as ``keep_activations`` says."""
+    if _takes(lin, x):
+        y, sums = _linear(x, lin.weight, lin.bias, want_sums, keep)
         return (y, sums if sums.numel() else None) if want_sums else y
+    kept_form(keep)
     return (lin(x), None) if want_sums else lin(x)
+
+
+def _batch_stats(block):
+    bn = block[1].batch_norm
+    return bn.training or bn.running_mean is None
+
+
+def _mlp_tail(seq, z, sums=None):
+    """What follows the first Linear of an MLP, from that Linear's output."""
+    for i, block in enumerate(seq):
+        bn, act = block[1].batch_norm, block[2]
+        if i + 1 == len(seq):
+            return batch_norm_act(z, bn, act, col_sums=sums)
+        if _batch_stats(seq[i + 1]):
+            z, sums = batch_norm_act_linear(z, bn, act, seq[i + 1][0], col_sums=sums, want_sums=True)
+        else:
+            z, sums = batch_norm_act_linear(z, bn, act, seq[i + 1][0], col_sums=sums), None
 
 
 def mlp(seq, x):
     """MLP of base_modules.py:38-48: per block Linear (streaming MFMA products,
     weight gradient by mvf_xty), then BatchNorm1d and the activation in one pair
     of kernels; in train mode the Linear leaves the column sums the batch
-    statistics are made of."""
-    for block in seq:
-        bn = block[1].batch_norm
-        if bn.training or bn.running_mean is None:
-            z, sums = linear(block[0], x, want_sums=True)
-        else:
-            z, sums = linear(block[0], x), None
-        x = batch_norm_act(z, bn, block[2], col_sums=sums)
-    return x
+    statistics are made of.  With 8-bit rows kept (``keep_activations``) an
+    activation and the Linear behind it share one packed copy."""
+    if len(seq) == 0:
+        return x
+    if _batch_stats(seq[0]):
+        z, sums = linear(seq[0][0], x, want_sums=True)
+    else:
+        z, sums = linear(seq[0][0], x), None
+    return _mlp_tail(seq, z, sums)
 
 
 def mlp_on_rows_and_sets(seq, x, x_set, ptr):
@@ -235,13 +487,11 @@ def mlp_on_rows_and_sets(seq, x, x_set, ptr):
     first Linear is split by columns, [x | x_set[seg]] W^T = x Wa^T + (x_set Wb^T + b)[seg],
     so the set features go through their half once per segment instead of once per row
     (DeepSetFeat's 'concatenation' fusion, pooling.py:669-681)."""
-    lin, bn, act = seq[0][0], seq[0][1].batch_norm, seq[0][2]
+    lin = seq[0][0]
     d = x.shape[1]
-    za = _Linear.apply(x, lin.weight[:, :d], None, False)[0]
-    zb = _Linear.apply(x_set, lin.weight[:, d:], lin.bias, False)[0]
-    z = za + P.gather_csr(zb, ptr)
-    y = batch_norm_act(z, bn, act)
-    return mlp(seq[1:], y) if len(seq) > 1 else y
+    za = _linear(x, lin.weight[:, :d], None)[0]
+    zb = _linear(x_set, lin.weight[:, d:], lin.bias)[0]
+    return _mlp_tail(seq, za + P.gather_csr(zb, ptr))
 
 
 def deep_set_feat(m, x, ptr):
