@@ -45,6 +45,14 @@ __device__ __forceinline__ unsigned r8_max8(unsigned v)
     return v;
 }
 
+// largest value of the 4 neighbouring lanes, in all of them
+__device__ __forceinline__ unsigned r8_max4(unsigned v)
+{
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, true));
+    return v;
+}
+
 __device__ __forceinline__ int r8_encode(float v, int e)
 {
     float q = rintf(ldexpf(v, R8_BIAS - e));
@@ -80,13 +88,30 @@ struct RowBF16 {
     static constexpr int E_MAX = R8_E_MAX;
     static __device__ __forceinline__ float get(T v) { return __uint_as_float((unsigned)v << 16); }
     static __device__ __forceinline__ T put(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }
+    static __device__ __forceinline__ unsigned put2(float a, float b)
+    {
+        typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+        const bf2 t = {(__bf16)a, (__bf16)b};
+        return __builtin_bit_cast(unsigned, t);
+    }
 };
 struct RowF16 {
     typedef unsigned short T;
     static constexpr int E_MAX = R8_E_MAX_F16;
     static __device__ __forceinline__ float get(T v) { return (float)__builtin_bit_cast(_Float16, v); }
     static __device__ __forceinline__ T put(float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
+    static __device__ __forceinline__ unsigned put2(float a, float b) { return (unsigned)put(a) | (unsigned)put(b) << 16; }
 };
+
+// Wide accesses at the alignment of one element: rows of a width that is no multiple of the vector
+// start anywhere, and the hardware reads and writes global memory at any address.
+typedef unsigned r8_u4 __attribute__((ext_vector_type(4)));
+typedef unsigned r8_u2 __attribute__((ext_vector_type(2)));
+struct __attribute__((packed, aligned(4))) R8Words4 { unsigned w[4]; };
+struct __attribute__((packed, aligned(2))) R8Half4 { unsigned w[2]; };
+struct __attribute__((packed, aligned(2))) R8Half8 { unsigned w[4]; };
+struct __attribute__((packed, aligned(1))) R8Bytes4 { unsigned w; };
+struct __attribute__((packed, aligned(1))) R8Bytes8 { unsigned w[2]; };
 
 // Four adjacent columns at col of a row of C columns (elements past C read as 0 and are not
 // written).  VEC: C % 4 == 0 and the base is aligned to four elements; then col + 3 < C too.
@@ -101,6 +126,16 @@ __device__ __forceinline__ void row_load4(const typename R::T *row, int col, int
             const uint2 t = *reinterpret_cast<const uint2 *>(row + col);
             v[0] = R::get((unsigned short)t.x); v[1] = R::get((unsigned short)(t.x >> 16));
             v[2] = R::get((unsigned short)t.y); v[3] = R::get((unsigned short)(t.y >> 16));
+        }
+    } else if (col + 4 <= C) {
+        if constexpr (sizeof(typename R::T) == 4) {
+            const R8Words4 t = *reinterpret_cast<const R8Words4 *>(row + col);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(t.w[j]);
+        } else {
+            const R8Half4 t = *reinterpret_cast<const R8Half4 *>(row + col);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = R::get((unsigned short)(t.w[j / 2] >> (16 * (j & 1))));
         }
     } else {
 #pragma unroll
@@ -120,6 +155,18 @@ __device__ __forceinline__ void row_store4(typename R::T *row, int col, int C, c
             t.y = (unsigned)R::put(v[2]) | (unsigned)R::put(v[3]) << 16;
             *reinterpret_cast<uint2 *>(row + col) = t;
         }
+    } else if (col + 4 <= C) {
+        if constexpr (sizeof(typename R::T) == 4) {
+            R8Words4 t;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t.w[j] = __float_as_uint(v[j]);
+            *reinterpret_cast<R8Words4 *>(row + col) = t;
+        } else {
+            R8Half4 t;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) t.w[j] = (unsigned)R::put(v[2 * j]) | (unsigned)R::put(v[2 * j + 1]) << 16;
+            *reinterpret_cast<R8Half4 *>(row + col) = t;
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -132,6 +179,8 @@ __device__ __forceinline__ unsigned codes_load4(const int8_t *row, int col, int 
 {
     if constexpr (VEC) {
         return *reinterpret_cast<const unsigned *>(row + col);
+    } else if (col + 4 <= C) {
+        return reinterpret_cast<const R8Bytes4 *>(row + col)->w;
     } else {
         unsigned w = 0;
 #pragma unroll
@@ -146,6 +195,8 @@ __device__ __forceinline__ void codes_store4(int8_t *row, int col, int C, unsign
 {
     if constexpr (VEC) {
         *reinterpret_cast<unsigned *>(row + col) = w;
+    } else if (col + 4 <= C) {
+        reinterpret_cast<R8Bytes4 *>(row + col)->w = w;
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
