@@ -210,5 +210,28 @@ def stream_ptr(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(index):
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def launch(device, fn, *args):
+    """``fn(*args, stream)`` on the current stream of ``device``, checked: a launch for
+    small inputs, where entering a device context and building a stream object would
+    take longer than the call.  Pointers are given as ``data_ptr()`` integers or None."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _stream_of(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream_of(index))
+    if rc != 0:
+        check(rc)
+
+
 def workspace(nbytes, device):
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)

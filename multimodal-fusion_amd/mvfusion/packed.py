@@ -48,10 +48,6 @@ class PackedRows:
         return f"PackedRows(shape={tuple(self.shape)}, dtype={self.dtype}, device={self.device})"
 
 
-def _groups(C):
-    return (C + GROUP - 1) // GROUP
-
-
 def _check_rows(x, what):
     if not x.is_cuda:
         raise RuntimeError(f"mvfusion {what} runs on a HIP device only (there is no CPU fallback).")
@@ -59,16 +55,20 @@ def _check_rows(x, what):
         raise TypeError(f"mvfusion {what} expects float32, bfloat16 or float16 rows, got {x.dtype}")
 
 
+def empty_codes(rows, C, device):
+    """Room for the 8-bit form of [rows, C]."""
+    return (torch.empty((rows, C), dtype=torch.int8, device=device),
+            torch.empty((rows, (C + GROUP - 1) // GROUP), dtype=torch.uint8, device=device))
+
+
 def pack_codes(x):
     """(codes, exps) of contiguous rows [rows, C] (``pack_rows`` without its checks)."""
     rows, C = x.shape
     dev = x.device
-    codes = torch.empty((rows, C), dtype=torch.int8, device=dev)
-    exps = torch.empty((rows, _groups(C)), dtype=torch.uint8, device=dev)
+    codes, exps = empty_codes(rows, C, dev)
     if rows:
-        with torch.cuda.device(dev):
-            L.check(L.load().mvf_pack_rows8(L.ptr(x), ROW_TYPES[x.dtype], rows, C, L.ptr(codes), L.ptr(exps),
-                                            L.stream_ptr(dev)))
+        L.launch(dev, L.load().mvf_pack_rows8, x.data_ptr(), ROW_TYPES[x.dtype], rows, C, codes.data_ptr(),
+                 exps.data_ptr())
     return codes, exps
 
 
@@ -88,14 +88,13 @@ def unpack_rows(codes, exps, dtype=torch.float32):
     if dtype not in ROW_TYPES:
         raise TypeError(f"mvfusion unpack_rows gives float32, bfloat16 or float16 rows, not {dtype}")
     if (codes.dtype != torch.int8 or exps.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] < 1
-            or exps.shape != (codes.shape[0], _groups(codes.shape[1])) or exps.device != codes.device):
+            or exps.shape != (codes.shape[0], (codes.shape[1] + GROUP - 1) // GROUP) or exps.device != codes.device):
         raise ValueError("unpack_rows expects int8 codes [rows, C] and uint8 exps [rows, ceil(C / 32)] on one device")
     codes, exps = codes.contiguous(), exps.contiguous()
     rows, C = codes.shape
     dev = codes.device
     y = torch.empty((rows, C), dtype=dtype, device=dev)
     if rows:
-        with torch.cuda.device(dev):
-            L.check(L.load().mvf_unpack_rows8(L.ptr(codes), L.ptr(exps), rows, C, L.ptr(y), ROW_TYPES[dtype],
-                                              L.stream_ptr(dev)))
+        L.launch(dev, L.load().mvf_unpack_rows8, codes.data_ptr(), exps.data_ptr(), rows, C, y.data_ptr(),
+                 ROW_TYPES[dtype])
     return y

@@ -32,17 +32,25 @@ def _norm_args(norm, C, x, name):
     if tuple(norm.normalized_shape) != (C,):
         raise ValueError(f"residual_norm: {name} normalises {tuple(norm.normalized_shape)}, the rows have {C} channels")
     eps = torch.finfo(x.dtype).eps if norm.eps is None else float(norm.eps)
-    return kind, _vector(norm.weight, C, x, name), _vector(getattr(norm, "bias", None), C, x, name), eps
+    params = norm._parameters
+    return kind, _vector(params["weight"], C, x, name), _vector(params.get("bias"), C, x, name), eps
 
 
 def _vector(t, C, x, name):
+    """t as C float32 values (autograd follows; t itself where it is that already)."""
     if t is None:
         return None
     if t.device != x.device:
         raise ValueError(f"residual_norm: {name} is on {t.device}, the rows are on {x.device}")
+    if t.dtype == torch.float32 and t.shape == (C,):
+        return t
     if not t.is_floating_point() or t.numel() not in (1, C):
         raise ValueError(f"residual_norm: {name} must hold 1 or {C} floating-point values, got {tuple(t.shape)} {t.dtype}")
     return t.float().reshape(-1).expand(C)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -63,20 +71,13 @@ class _ResidualNorm(torch.autograd.Function):
         h = torch.empty_like(x) if pre else None
         wants = keep is not None
         keep8 = keep == "int8"
-        xq = fq = (None, None)
-        if keep8:
-            def codes():
-                return (torch.empty((rows, C), dtype=torch.int8, device=dev),
-                        torch.empty((rows, packed._groups(C)), dtype=torch.uint8, device=dev))
-            xq = codes() if pre else xq
-            fq = codes() if f is not None else fq
+        xq = packed.empty_codes(rows, C, dev) if keep8 and pre else (None, None)
+        fq = packed.empty_codes(rows, C, dev) if keep8 and f is not None else (None, None)
         stats = torch.empty((4, rows), dtype=torch.float32, device=dev) if wants and (pre or post) else None
-        with torch.cuda.device(dev):
-            L.check(lib.mvf_residual_norm_forward(
-                L.ptr(x), L.ptr(f), packed.ROW_TYPES[x.dtype], rows, C, L.ptr(gate), G, L.ptr(seen), L.ptr(scale),
-                post, L.ptr(w_post), L.ptr(b_post), eps_post, pre, L.ptr(w_pre), L.ptr(b_pre), eps_pre,
-                L.ptr(out), L.ptr(h), L.ptr(xq[0]), L.ptr(xq[1]), L.ptr(fq[0]), L.ptr(fq[1]), L.ptr(stats),
-                L.stream_ptr(dev)))
+        L.launch(dev, lib.mvf_residual_norm_forward, x.data_ptr(), _addr(f), packed.ROW_TYPES[x.dtype], rows, C,
+                 _addr(gate), G, _addr(seen), _addr(scale), post, _addr(w_post), _addr(b_post), eps_post,
+                 pre, _addr(w_pre), _addr(b_pre), eps_pre, out.data_ptr(), _addr(h), _addr(xq[0]), _addr(xq[1]),
+                 _addr(fq[0]), _addr(fq[1]), _addr(stats))
         if wants:
             ctx.set_materialize_grads(False)
             ctx.save_for_backward(
@@ -107,12 +108,10 @@ class _ResidualNorm(torch.autograd.Function):
         vectors = [empty(need[i], (C,)) for i in range(3, 8)]
         nbytes = lib.mvf_residual_norm_workspace_bytes(rows, C) if any(need[3:8]) else 0
         ws = L.workspace(nbytes, dev) if nbytes else None
-        with torch.cuda.device(dev):
-            L.check(lib.mvf_residual_norm_backward(
-                L.ptr(d_out), L.ptr(d_h), L.ptr(x), L.ptr(xc), L.ptr(xe), L.ptr(f), L.ptr(fc), L.ptr(fe),
-                packed.ROW_TYPES[dtype], rows, C, L.ptr(gate), G, L.ptr(seen), L.ptr(scale),
-                post, L.ptr(w_post), L.ptr(b_post), pre, L.ptr(w_pre), L.ptr(stats), L.ptr(dx), L.ptr(df),
-                L.ptr(dgate), *(L.ptr(v) for v in vectors), L.ptr(ws), nbytes, L.stream_ptr(dev)))
+        L.launch(dev, lib.mvf_residual_norm_backward, _addr(d_out), _addr(d_h), _addr(x), _addr(xc), _addr(xe),
+                 _addr(f), _addr(fc), _addr(fe), packed.ROW_TYPES[dtype], rows, C, _addr(gate), G, _addr(seen),
+                 _addr(scale), post, _addr(w_post), _addr(b_post), pre, _addr(w_pre), _addr(stats), _addr(dx),
+                 _addr(df), _addr(dgate), *map(_addr, vectors), _addr(ws), nbytes)
         return (dx, df, dgate, *vectors) + nothing[8:]
 
 
@@ -148,7 +147,8 @@ def residual_norm(x, f, post=None, pre=None, gate=None, scale=None, seen=None, k
                          f"x is {tuple(shape)} {x.dtype} on {x.device}")
     k_post, w_post, b_post, eps_post = _norm_args(post, C, x, "post")
     k_pre, w_pre, b_pre, eps_pre = _norm_args(pre, C, x, "pre")
-    rows = x.reshape(-1, C)
+    flat = x.dim() == 2         # (views only where they are needed: each is a node of the graph)
+    rows = x if flat else x.reshape(-1, C)
     if gate is not None:
         if gate.device != x.device or not gate.is_floating_point():
             raise ValueError("residual_norm: gate must hold floating-point values on the device of the rows")
@@ -157,7 +157,7 @@ def residual_norm(x, f, post=None, pre=None, gate=None, scale=None, seen=None, k
         if gate.shape[:-1] != shape[:-1] or gate.dim() != len(shape) or gate.shape[-1] < 1 or C % gate.shape[-1] != 0:
             raise ValueError(f"residual_norm: gate {tuple(gate.shape)} does not fit rows {tuple(shape)}: one value per "
                              f"row and channel group, in a number of groups that divides {C}")
-        gate = gate.float().reshape(-1, gate.shape[-1])
+        gate = gate.float() if flat else gate.float().reshape(-1, gate.shape[-1])
     if scale is not None:
         if not torch.is_tensor(scale):
             scale = torch.full((C,), float(scale), dtype=torch.float32, device=x.device)
@@ -165,13 +165,14 @@ def residual_norm(x, f, post=None, pre=None, gate=None, scale=None, seen=None, k
     if seen is not None:
         if seen.dtype != torch.bool or seen.shape != shape[:-1] or seen.device != x.device:
             raise ValueError(f"residual_norm: seen must be a bool tensor {tuple(shape[:-1])} on the device of the rows")
-        seen = seen.reshape(-1).contiguous().view(torch.uint8)
-    flat = None if f is None else f.reshape(-1, C)
-    leaves = (rows, flat, gate, scale, w_post, b_post, w_pre, b_pre)
+        seen = (seen if flat else seen.reshape(-1)).contiguous()
+    if f is not None and not flat:
+        f = f.reshape(-1, C)
+    leaves = (rows, f, gate, scale, w_post, b_post, w_pre, b_pre)
     keep = training.kept_form(keep)
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves)):
         keep = None
     got = _ResidualNorm.apply(*leaves, seen, k_post, k_pre, eps_post, eps_pre, keep)
-    if k_pre:
-        return got[0].view(shape), got[1].view(shape)
-    return got.view(shape)
+    if flat:
+        return got
+    return (got[0].view(shape), got[1].view(shape)) if k_pre else got.view(shape)

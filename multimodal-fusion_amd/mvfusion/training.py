@@ -123,23 +123,24 @@ class _BatchNormAct(torch.autograd.Function):
         return gz, gw, gb, None, None, None, None, None, None, None
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _bn8_forward(z, weight, bias, rm, rv, eps, slope, batch_stats, factor, col_sums):
     """(y, codes, exps, invstd) of mvf_batch_norm_act8_forward."""
     lib = L.load()
     rows, C = z.shape
     dev = z.device
     y = torch.empty_like(z)
-    codes = torch.empty((rows, C), dtype=torch.int8, device=dev)
-    exps = torch.empty((rows, packed._groups(C)), dtype=torch.uint8, device=dev)
+    codes, exps = packed.empty_codes(rows, C, dev)
     invstd = torch.empty(C, dtype=torch.float32, device=dev)
     nbytes = lib.mvf_batch_norm_act8_workspace_bytes(C)
     ws = L.workspace(nbytes, dev)
-    with torch.cuda.device(dev):
-        L.check(lib.mvf_batch_norm_act8_forward(
-            L.ptr(z), rows, C, L.ptr(weight), L.ptr(bias), L.ptr(rm), L.ptr(rv), int(batch_stats),
-            float(factor), float(eps), int(slope is not None), 0.0 if slope is None else float(slope),
-            L.ptr(y), L.ptr(codes), L.ptr(exps), L.ptr(invstd),
-            L.ptr(col_sums), 0 if col_sums is None else col_sums.shape[0], L.ptr(ws), nbytes, L.stream_ptr(dev)))
+    L.launch(dev, lib.mvf_batch_norm_act8_forward, z.data_ptr(), rows, C, _addr(weight), _addr(bias), _addr(rm),
+             _addr(rv), batch_stats, factor, eps, slope is not None, slope or 0.0, y.data_ptr(), codes.data_ptr(),
+             exps.data_ptr(), invstd.data_ptr(), _addr(col_sums), 0 if col_sums is None else col_sums.shape[0],
+             ws.data_ptr(), nbytes)
     return y, codes, exps, invstd
 
 
@@ -154,16 +155,14 @@ def _bn8_backward(grad_y, codes, exps, weight, bias, invstd, batch_stats, slope,
     gb = torch.empty(C, dtype=torch.float32, device=dev) if needs[2] else None
     nbytes = lib.mvf_batch_norm_act8_workspace_bytes(C)
     ws = L.workspace(nbytes, dev)
-    with torch.cuda.device(dev):
-        L.check(lib.mvf_batch_norm_act8_backward(
-            L.ptr(grad_y), L.ptr(codes), L.ptr(exps), rows, C, L.ptr(weight), L.ptr(bias), L.ptr(invstd),
-            int(batch_stats), int(slope is not None), 0.0 if slope is None else float(slope),
-            L.ptr(gz), L.ptr(gw), L.ptr(gb), L.ptr(ws), nbytes, L.stream_ptr(dev)))
+    L.launch(dev, lib.mvf_batch_norm_act8_backward, grad_y.data_ptr(), codes.data_ptr(), exps.data_ptr(), rows, C,
+             _addr(weight), _addr(bias), invstd.data_ptr(), batch_stats, slope is not None, slope or 0.0,
+             _addr(gz), _addr(gw), _addr(gb), ws.data_ptr(), nbytes)
     return gz, gw, gb
 
 
 def _vector(t):
-    return None if t is None else t.detach().float().contiguous()
+    return None if t is None else t.detach().contiguous()
 
 
 class _BatchNormAct8(torch.autograd.Function):
@@ -388,11 +387,9 @@ def xty8(x, codes, exps, tail=None, want_sums=False):
     w, b, slope = tail if tail is not None else (None, None, None)
     nbytes = lib.mvf_xty8_workspace_bytes()
     ws = L.workspace(nbytes, dev)
-    with torch.cuda.device(dev):
-        L.check(lib.mvf_xty8(
-            L.ptr(x), A, A, L.ptr(codes), L.ptr(exps), B, x.shape[0], int(tail is not None), L.ptr(w), L.ptr(b),
-            int(slope is not None), 0.0 if slope is None else float(slope), L.ptr(out), B, L.ptr(sums), L.ptr(ws),
-            nbytes, L.stream_ptr(dev)))
+    L.launch(dev, lib.mvf_xty8, x.data_ptr(), A, A, codes.data_ptr(), exps.data_ptr(), B, x.shape[0],
+             tail is not None, _addr(w), _addr(b), slope is not None, slope or 0.0, out.data_ptr(), B, _addr(sums),
+             ws.data_ptr(), nbytes)
     return out, sums
 
 
