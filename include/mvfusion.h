@@ -549,6 +549,39 @@ int mvf_xty8(
     int32_t tail, const float *bn_weight, const float *bn_bias, int32_t act, float slope,
     float *out, int32_t ldo, float *x_sums, void *workspace, size_t workspace_bytes, void *stream);
 
+/* y = x W^T (+ bias) for contiguous float32 rows, with the 8-bit rows of x, in one pass; and from one
+ * read of grad_y: grad_x = grad_y W, grad_weight = grad_y^T xq with xq as read back, grad_bias (may
+ * be NULL) = the column sums of grad_y.  I in {8, 16, 32, 64}, O a multiple of 8 up to 64
+ * (mvf_linear_rows8_supported); x, y, grad_y and grad_x 16-byte aligned, weight [O][I] contiguous.  y has
+ * the bits of mvf_linear_rows; col_sums / n_col_sums as in mvf_linear_rows_sums (NULL: not
+ * wanted).  workspace: mvf_xty8_workspace_bytes().  Sums over rows in a fixed order. */
+int mvf_linear_rows8_supported(int32_t I, int32_t O);
+int mvf_linear_rows8_forward(
+    const float *x, int32_t I, const float *weight, const float *bias, int32_t O, int64_t rows, float *y,
+    int8_t *codes, uint8_t *exps, double *col_sums, size_t col_sums_bytes, int32_t *n_col_sums, void *stream);
+int mvf_linear_rows8_backward(
+    const float *grad_y, const int8_t *codes, const uint8_t *exps, const float *weight, int32_t I, int32_t O, int64_t rows,
+    float *grad_x, float *grad_weight, float *grad_bias, void *workspace, size_t workspace_bytes, void *stream);
+
+/* BatchNorm + LeakyReLU (mvf_batch_norm_act8_forward) and the Linear behind it in one pass over z (two
+ * with batch statistics that no col_sums bring): the activated rows are never stored, and the codes are
+ * all that the backward keeps of a row.  Shapes and alignment as for mvf_linear_rows8_*; y_sums /
+ * n_y_sums: column sums of y (NULL: not wanted).  backward: two passes over grad_y and the codes,
+ * grad_y W is formed in both and stored in none; grad_z, grad_bn_weight, grad_bn_bias and grad_bias may
+ * be NULL.  workspace: mvf_batch_norm_act_linear8_workspace_bytes(I) in both directions. */
+size_t mvf_batch_norm_act_linear8_workspace_bytes(int32_t I);
+int mvf_batch_norm_act_linear8_forward(
+    const float *z, int64_t rows, int32_t I, const float *bn_weight, const float *bn_bias,
+    float *running_mean, float *running_var, int32_t training, float momentum, float eps, int32_t act, float slope,
+    const float *weight, const float *bias, int32_t O, float *y, int8_t *codes, uint8_t *exps, float *save_invstd,
+    const double *col_sums, int32_t n_col_sums, double *y_sums, size_t y_sums_bytes, int32_t *n_y_sums,
+    void *workspace, size_t workspace_bytes, void *stream);
+int mvf_batch_norm_act_linear8_backward(
+    const float *grad_y, const int8_t *codes, const uint8_t *exps, int64_t rows, int32_t I, const float *bn_weight,
+    const float *bn_bias, const float *save_invstd, int32_t training, int32_t act, float slope, const float *weight, int32_t O,
+    float *grad_z, float *grad_bn_weight, float *grad_bn_bias, float *grad_weight, float *grad_bias,
+    void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---------------------------------------------------------------------- *
  * Gated residual block between two norms, e.g. a pooled image feature f onto the
  * point's own feature x (the residual fusion behind the pools, with a gate per

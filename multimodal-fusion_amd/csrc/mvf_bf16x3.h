@@ -1,0 +1,50 @@
+// float32 values as exact sums of bf16 parts for the bf16 matrix cores (v_mfma_f32_32x32x16_bf16), and
+// the fold of per-workgroup partial results, shared by the weight-gradient kernels.
+#pragma once
+
+#include "mvf_common.h"
+
+namespace mvf {
+
+typedef float xty_acc __attribute__((ext_vector_type(16)));
+typedef __bf16 xty_bf8 __attribute__((ext_vector_type(8)));
+typedef unsigned xty_u4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ xty_acc xty_mfma16(xty_u4 a, xty_u4 b, xty_acc c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(xty_bf8, a), __builtin_bit_cast(xty_bf8, b), c, 0, 0, 0);
+}
+
+// high halves of two floats as two bf16 (the first in the low half)
+__device__ __forceinline__ unsigned xty_hi2(float a, float b)
+{
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+
+// 8 float32 as bf16 parts: v = p[0] + p[1] + p[2] exactly for PARTS == 3, p[0] alone for values that
+// one bf16 holds
+template <int PARTS> struct XtyParts {
+    xty_u4 p[PARTS];
+    __device__ __forceinline__ void cut(const float (&v)[8])
+    {
+        float r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = v[j];
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) p[k][h] = xty_hi2(r[2 * h], r[2 * h + 1]);
+            if (k + 1 < PARTS)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[j] -= __uint_as_float(__float_as_uint(r[j]) & 0xffff0000u);
+        }
+    }
+};
+
+// Adds up the partial results of nwg workgroups: partial [nwg][NA * NB * 1024] accumulators of NA x NB
+// blocks of 32 x 32 sums as v_mfma_f32_32x32x16_bf16 leaves them (vx / vy: an operand of two blocks holds
+// columns 2 n and 2 n + 1 in lane n), out [A][ldo], and with partial_sums [nwg][64] the sums [A].
+void xty8_fold(const float *partial, const float *partial_sums, int nwg, int NA, int NB, int vx, int vy, int A, int B,
+               float *out, int ldo, float *sums, hipStream_t st);
+
+}  // namespace mvf

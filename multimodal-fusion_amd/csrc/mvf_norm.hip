@@ -15,12 +15,12 @@
 // per block; a second small kernel folds the partials in a fixed order, so the
 // statistics are the same on every run.
 #include "mvf_bn_kink.h"
+#include "mvf_norm.h"
 #include "mvf_rows8.h"
 
 namespace mvf {
 
 constexpr int BN_THREADS = 256;
-constexpr int BN_MAX_BLOCKS = 1024;
 constexpr int BN8_MAX_BLOCKS = 4096;
 constexpr int BN_FOLD_COLS = 4;         // columns per block of the fold kernels
 
@@ -717,6 +717,44 @@ extern "C" size_t mvf_batch_norm_act8_workspace_bytes(int32_t C)
     return mvf_batch_norm_act_workspace_bytes(C) + align_up(2 * (size_t)C * sizeof(double));
 }
 
+namespace mvf {
+
+Bn8Workspace bn8_workspace(void *workspace, int C)
+{
+    char *p = (char *)workspace;
+    return {(double *)p, (float *)(p + bn_partial_bytes(C)), (double *)(p + mvf_batch_norm_act_workspace_bytes(C))};
+}
+
+void bn8_statistics(const float *z, i64 rows, int C, float *running_mean, float *running_var, int training, float momentum,
+                    float eps, const double *col_sums, int n_col_sums, const Bn8Workspace &w, float *save_invstd, hipStream_t st)
+{
+    if (!training) {
+        hipLaunchKernelGGL(bn_running_terms_kernel, dim3(cdiv(C, 256)), dim3(256), 0, st, (const float *)running_mean,
+                           (const float *)running_var, C, eps, w.terms, save_invstd, w.terms64);
+        return;
+    }
+    const double *partial = col_sums;
+    int nblk = n_col_sums;
+    if (!col_sums) {
+        const bool vec = C % 4 == 0 && (uintptr_t)z % 16 == 0;
+        const BnGrid g = bn_grid(rows, C, vec ? 4 : 1);
+        if (vec) hipLaunchKernelGGL(bn_sums_kernel<4>, g.grid, dim3(BN_THREADS), 0, st, z, rows, C, g.rows_per_block, w.partial);
+        else hipLaunchKernelGGL(bn_sums_kernel<1>, g.grid, dim3(BN_THREADS), 0, st, z, rows, C, g.rows_per_block, w.partial);
+        partial = w.partial;
+        nblk = g.nblk;
+    }
+    hipLaunchKernelGGL(bn_stats_kernel, dim3(cdiv(C, BN_FOLD_COLS)), dim3(BN_THREADS), 0, st, partial, nblk, C, rows, eps,
+                       momentum, running_mean, running_var, w.terms, save_invstd, w.terms64);
+}
+
+void bn8_grad_terms(const Bn8Workspace &w, int nblk, int C, i64 rows, float *grad_weight, float *grad_bias, hipStream_t st)
+{
+    hipLaunchKernelGGL(bn_grad_terms_kernel, dim3(cdiv(C, BN_FOLD_COLS)), dim3(BN_THREADS), 0, st, (const double *)w.partial,
+                       nblk, C, rows, grad_weight, grad_bias, w.terms);
+}
+
+}  // namespace mvf
+
 extern "C" int mvf_batch_norm_act8_forward(
     const float *z, int64_t rows, int32_t C, const float *weight, const float *bias,
     float *running_mean, float *running_var, int32_t training, float momentum, float eps,
@@ -732,36 +770,19 @@ extern "C" int mvf_batch_norm_act8_forward(
                 "batch_norm_act8_forward: workspace too small");
     MVF_REQUIRE(!col_sums || n_col_sums >= 1, "batch_norm_act8_forward: column sums without partial rows");
     hipStream_t st = (hipStream_t)stream;
-    double *mine = (double *)workspace;
-    float *mean = (float *)((char *)workspace + bn_partial_bytes(C));
-    double *terms64 = (double *)((char *)workspace + mvf_batch_norm_act_workspace_bytes(C));
-    if (training) {
-        const double *partial = col_sums;
-        int nblk = n_col_sums;
-        if (!col_sums) {
-            const bool vec = C % 4 == 0 && (uintptr_t)z % 16 == 0;
-            const BnGrid g = bn_grid(rows, C, vec ? 4 : 1);
-            if (vec) hipLaunchKernelGGL(bn_sums_kernel<4>, g.grid, dim3(BN_THREADS), 0, st, z, (i64)rows, C, g.rows_per_block, mine);
-            else hipLaunchKernelGGL(bn_sums_kernel<1>, g.grid, dim3(BN_THREADS), 0, st, z, (i64)rows, C, g.rows_per_block, mine);
-            partial = mine;
-            nblk = g.nblk;
-        }
-        hipLaunchKernelGGL(bn_stats_kernel, dim3(cdiv(C, BN_FOLD_COLS)), dim3(BN_THREADS), 0, st,
-                           partial, nblk, C, (i64)rows, eps, momentum,
-                           running_mean, running_var, mean, save_invstd, terms64);
-    } else {
-        hipLaunchKernelGGL(bn_running_terms_kernel, dim3(cdiv(C, 256)), dim3(256), 0, st,
-                           (const float *)running_mean, (const float *)running_var, C, eps, mean, save_invstd, terms64);
-    }
+    const Bn8Workspace w = bn8_workspace(workspace, C);
+    bn8_statistics(z, rows, C, running_mean, running_var, training, momentum, eps, col_sums, n_col_sums, w, save_invstd, st);
+    const float *mean = w.terms;
+    const double *terms64 = w.terms64;
     const bool vec = C % 4 == 0 && (uintptr_t)z % 16 == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)codes % 4 == 0;
     const R8Grid g = r8_grid(rows, C, true, 4, BN8_MAX_BLOCKS);
     if (vec)
         hipLaunchKernelGGL(bn_apply8_kernel<true>, g.grid, dim3(BN_THREADS), 0, st, z, (i64)rows, C, g.rows_per_block,
-                           (const float *)mean, (const float *)save_invstd, (const double *)terms64, weight, bias,
+                           mean, (const float *)save_invstd, terms64, weight, bias,
                            act, slope, y, codes, exps);
     else
         hipLaunchKernelGGL(bn_apply8_kernel<false>, g.grid, dim3(BN_THREADS), 0, st, z, (i64)rows, C, g.rows_per_block,
-                           (const float *)mean, (const float *)save_invstd, (const double *)terms64, weight, bias,
+                           mean, (const float *)save_invstd, terms64, weight, bias,
                            act, slope, y, codes, exps);
     MVF_LAUNCH_CHECK();
     return MVF_OK;
@@ -780,8 +801,9 @@ extern "C" int mvf_batch_norm_act8_backward(
     hipStream_t st = (hipStream_t)stream;
     const bool vec = C % 4 == 0 && (uintptr_t)grad_y % 16 == 0 && (uintptr_t)grad_z % 16 == 0 && (uintptr_t)codes % 4 == 0;
     const BnGrid g = bn_grid(rows, C, vec ? 4 : 1);
-    double *partial = (double *)workspace;
-    float *col_terms = (float *)((char *)workspace + bn_partial_bytes(C));
+    const Bn8Workspace ws8 = bn8_workspace(workspace, C);
+    double *partial = ws8.partial;
+    float *col_terms = ws8.terms;
     if ((training && grad_z) || grad_weight || grad_bias) {
         if (vec)
             hipLaunchKernelGGL(bn_grad_sums8_kernel<4>, g.grid, dim3(BN_THREADS), 0, st, grad_y, codes, exps, (i64)rows, C,
@@ -789,8 +811,7 @@ extern "C" int mvf_batch_norm_act8_backward(
         else
             hipLaunchKernelGGL(bn_grad_sums8_kernel<1>, g.grid, dim3(BN_THREADS), 0, st, grad_y, codes, exps, (i64)rows, C,
                                g.rows_per_block, weight, bias, act, slope, partial);
-        hipLaunchKernelGGL(bn_grad_terms_kernel, dim3(cdiv(C, BN_FOLD_COLS)), dim3(BN_THREADS), 0, st,
-                           (const double *)partial, g.nblk, C, (i64)rows, grad_weight, grad_bias, col_terms);
+        bn8_grad_terms(ws8, g.nblk, C, rows, grad_weight, grad_bias, st);
     }
     if (grad_z) {
         if (vec)

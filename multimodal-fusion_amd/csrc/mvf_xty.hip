@@ -14,6 +14,7 @@
 // every workgroup writes one partial result and a second kernel adds the partials in workgroup
 // order: no atomics, the same bits on every run.  The pass is bound by HBM (4 (A + B) bytes per
 // row).
+#include "mvf_bf16x3.h"
 #include "mvf_bn_kink.h"
 #include "mvf_rows8.h"
 
@@ -23,7 +24,6 @@ constexpr int XTY_THREADS = 256;
 constexpr int XTY_WAVES = XTY_THREADS / 64;
 constexpr int XTY_MAX_WGS = 1024;       // partial results in the workspace
 
-typedef float xty_acc __attribute__((ext_vector_type(16)));
 typedef float xty_f2 __attribute__((ext_vector_type(2)));
 // pointers into global memory that went through integer arithmetic (a generic pointer would load
 // with flat instructions, which wait on both memory counters)
@@ -265,42 +265,8 @@ __global__ __launch_bounds__(XTY_FOLD_SLOTS * XTY_FOLD_SLICES) void xty_fold_ker
 // Operands come straight from global memory: lane (n, kh) owns columns of a block and the 8 rows
 // 8 kh .. 8 kh + 7 of a step of 16, 128 to 256 contiguous bytes per row and load.  Steps are dealt to
 // the waves in turn; one step is in flight while the one before is cut and multiplied.
-typedef __bf16 xty_bf8 __attribute__((ext_vector_type(8)));
-typedef unsigned xty_u4 __attribute__((ext_vector_type(4)));
-
 constexpr int XTY8_STEP = 16;
 constexpr int XTY8_WGS = 2;          // workgroups per compute unit
-
-__device__ __forceinline__ xty_acc xty_mfma16(xty_u4 a, xty_u4 b, xty_acc c)
-{
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(xty_bf8, a), __builtin_bit_cast(xty_bf8, b), c, 0, 0, 0);
-}
-
-// high halves of two floats as two bf16 (the first in the low half)
-__device__ __forceinline__ unsigned xty_hi2(float a, float b)
-{
-    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-}
-
-// 8 float32 as bf16 parts: v = p[0] + p[1] + p[2] exactly for PARTS == 3, p[0] alone for values that
-// one bf16 holds
-template <int PARTS> struct XtyParts {
-    xty_u4 p[PARTS];
-    __device__ __forceinline__ void cut(const float (&v)[8])
-    {
-        float r[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = v[j];
-#pragma unroll
-        for (int k = 0; k < PARTS; ++k) {
-#pragma unroll
-            for (int h = 0; h < 4; ++h) p[k][h] = xty_hi2(r[2 * h], r[2 * h + 1]);
-            if (k + 1 < PARTS)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) r[j] -= __uint_as_float(__float_as_uint(r[j]) & 0xffff0000u);
-        }
-    }
-};
 
 struct XtyTail {            // TAIL: the column terms of y = act(gamma * zq + beta)
     const float *weight, *bias;     // may be NULL (1 and 0)
@@ -534,6 +500,14 @@ __global__ __launch_bounds__(XTY_FOLD_SLOTS * XTY_FOLD_SLICES) void xty8_fold_ke
     if (a < A && b < B) out[(size_t)a * ldo + b] = (float)s;
 }
 
+void xty8_fold(const float *partial, const float *partial_sums, int nwg, int NA, int NB, int vx, int vy, int A, int B,
+               float *out, int ldo, float *sums, hipStream_t st)
+{
+    hipLaunchKernelGGL(xty8_fold_kernel, dim3(NA * NB * 1024 / XTY_FOLD_SLOTS + (sums ? 64 / XTY_FOLD_SLOTS : 0)),
+                       dim3(XTY_FOLD_SLOTS * XTY_FOLD_SLICES), 0, st, partial, partial_sums, nwg, NA, NB, vx, vy, A, B,
+                       out, ldo, sums);
+}
+
 __global__ void xty8_zero_kernel(float *out, int A, int B, int ldo, float *sums)
 {
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
@@ -672,10 +646,8 @@ extern "C" int mvf_xty8(
             else MVF_XTY8_T(2, 2, false, false);
 #undef MVF_XTY8_T
 #undef MVF_XTY8_LAUNCH
-            hipLaunchKernelGGL(xty8_fold_kernel, dim3(NA * NB * 1024 / XTY_FOLD_SLOTS + (want ? 64 / XTY_FOLD_SLOTS : 0)),
-                               dim3(XTY_FOLD_SLOTS * XTY_FOLD_SLICES), 0, st, (const float *)partial,
-                               (const float *)partial_sums, (int)nwg, NA, NB, (int)vx, (int)vq, At, Bt,
-                               out + (size_t)a0 * ldo + b0, (int)ldo, want ? x_sums + a0 : nullptr);
+            xty8_fold(partial, partial_sums, (int)nwg, NA, NB, (int)vx, (int)vq, At, Bt, out + (size_t)a0 * ldo + b0,
+                      (int)ldo, want ? x_sums + a0 : nullptr, st);
         }
     MVF_LAUNCH_CHECK();
     return MVF_OK;

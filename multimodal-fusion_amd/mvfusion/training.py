@@ -19,8 +19,9 @@ Inside ``keep_activations('int8')`` (or with ``keep='int8'``) the dense layers k
 8-bit rows (``packed``) for their backward instead of float32 ones: a Linear the
 rows it got, BatchNorm + LeakyReLU its normalised rows, and a Linear behind such
 an activation nothing of its own: its weight gradient is made of the packed
-rows of the activation.  The forward is the same bit for bit; gradients are the
-formulas' on the rows as they read back.
+rows of the activation.  The forward computes the same (the order of a product's
+sum may differ below 4096 rows); gradients are the formulas' on the rows as they
+read back.
 
 The computation follows modules/multimodal/pooling.py: ``DeepSetFeat.forward``
 :658-681, ``MinMaxDiffSetFeat.forward`` :577-597, ``MLPSetFeat.forward``
@@ -165,6 +166,84 @@ def _vector(t):
     return None if t is None else t.detach().contiguous()
 
 
+def _fused8(rows, weight):
+    """Do the kernels that pack rows within a Linear's own pass take these?"""
+    return bool(L.load().mvf_linear_rows8_supported(weight.shape[1], weight.shape[0])) and rows.data_ptr() % 16 == 0
+
+
+def _sums_buffer(lib, cout, want, dev):
+    nbytes = lib.mvf_linear_rows_sums_bytes(cout) if want else 0
+    return torch.empty(nbytes // 8, dtype=torch.float64, device=dev) if want else None, nbytes, ctypes.c_int32(0)
+
+
+def _linear8_forward(x, weight, bias, want_sums):
+    """(y, codes, exps, partial column sums or None) of mvf_linear_rows8_forward."""
+    lib = L.load()
+    rows, (cout, cin), dev = x.shape[0], weight.shape, x.device
+    weight, bias = _vector(weight), _vector(bias)
+    y = torch.empty((rows, cout), dtype=torch.float32, device=dev)
+    codes, exps = packed.empty_codes(rows, cin, dev)
+    sums, nbytes, n = _sums_buffer(lib, cout, want_sums, dev)
+    L.launch(dev, lib.mvf_linear_rows8_forward, x.data_ptr(), cin, weight.data_ptr(), _addr(bias), cout, rows,
+             y.data_ptr(), codes.data_ptr(), exps.data_ptr(), _addr(sums), nbytes, ctypes.addressof(n))
+    return y, codes, exps, sums[:n.value * 2 * cout].view(n.value, 2, cout) if want_sums else None
+
+
+def _linear8_backward(grad_y, codes, exps, weight, want_bias):
+    """(grad_x, grad_weight, grad_bias or None) of mvf_linear_rows8_backward."""
+    lib = L.load()
+    rows, (cout, cin), dev = grad_y.shape[0], weight.shape, grad_y.device
+    weight = _vector(weight)
+    gx = torch.empty((rows, cin), dtype=torch.float32, device=dev)
+    gw = torch.empty((cout, cin), dtype=torch.float32, device=dev)
+    gb = torch.empty(cout, dtype=torch.float32, device=dev) if want_bias else None
+    nbytes = lib.mvf_xty8_workspace_bytes()
+    ws = L.workspace(nbytes, dev)
+    L.launch(dev, lib.mvf_linear_rows8_backward, grad_y.data_ptr(), codes.data_ptr(), exps.data_ptr(),
+             weight.data_ptr(), cin, cout, rows, gx.data_ptr(), gw.data_ptr(), _addr(gb), ws.data_ptr(), nbytes)
+    return gx, gw, gb
+
+
+def _bn_linear8_forward(z, w, b, rm, rv, eps, slope, batch_stats, factor, col_sums, weight, bias, want_sums):
+    """(out, codes, exps, invstd, partial column sums or None) of mvf_batch_norm_act_linear8_forward."""
+    lib = L.load()
+    rows, (cout, cin), dev = z.shape[0], weight.shape, z.device
+    weight, bias = _vector(weight), _vector(bias)
+    out = torch.empty((rows, cout), dtype=torch.float32, device=dev)
+    codes, exps = packed.empty_codes(rows, cin, dev)
+    invstd = torch.empty(cin, dtype=torch.float32, device=dev)
+    sums, sbytes, n = _sums_buffer(lib, cout, want_sums, dev)
+    nbytes = lib.mvf_batch_norm_act_linear8_workspace_bytes(cin)
+    ws = L.workspace(nbytes, dev)
+    L.launch(dev, lib.mvf_batch_norm_act_linear8_forward, z.data_ptr(), rows, cin, _addr(w), _addr(b), _addr(rm),
+             _addr(rv), batch_stats, factor, eps, slope is not None, slope or 0.0, weight.data_ptr(), _addr(bias), cout,
+             out.data_ptr(), codes.data_ptr(), exps.data_ptr(), invstd.data_ptr(), _addr(col_sums),
+             0 if col_sums is None else col_sums.shape[0], _addr(sums), sbytes, ctypes.addressof(n),
+             ws.data_ptr(), nbytes)
+    return out, codes, exps, invstd, sums[:n.value * 2 * cout].view(n.value, 2, cout) if want_sums else None
+
+
+def _bn_linear8_backward(grad_out, codes, exps, w, b, invstd, batch_stats, slope, weight, needs):
+    """Gradients of (z, BatchNorm's weight and bias, the Linear's weight and bias), those of `needs`, by
+    mvf_batch_norm_act_linear8_backward."""
+    lib = L.load()
+    (rows, cin), cout, dev = codes.shape, weight.shape[0], codes.device
+    weight = _vector(weight)
+
+    def empty(wanted, *shape):
+        return torch.empty(shape, dtype=torch.float32, device=dev) if wanted else None
+
+    gz, gw, gb = empty(True, rows, cin), empty(needs[1], cin), empty(needs[2], cin)
+    glw, glb = empty(True, cout, cin), empty(needs[4], cout)
+    nbytes = lib.mvf_batch_norm_act_linear8_workspace_bytes(cin)
+    ws = L.workspace(nbytes, dev)
+    L.launch(dev, lib.mvf_batch_norm_act_linear8_backward, grad_out.data_ptr(), codes.data_ptr(), exps.data_ptr(), rows,
+             cin, _addr(w), _addr(b), invstd.data_ptr(), batch_stats, slope is not None, slope or 0.0,
+             weight.data_ptr(), cout, gz.data_ptr(), _addr(gw), _addr(gb), glw.data_ptr(), _addr(glb),
+             ws.data_ptr(), nbytes)
+    return gz, gw, gb, glw, glb
+
+
 class _BatchNormAct8(torch.autograd.Function):
     """_BatchNormAct that keeps the normalised rows in 8 bits."""
 
@@ -193,13 +272,18 @@ class _BatchNormActLinear8(torch.autograd.Function):
     def forward(ctx, z, bn_weight, bn_bias, weight, bias, rm, rv, eps, slope, batch_stats, factor, col_sums,
                 want_sums):
         w, b = _vector(bn_weight), _vector(bn_bias)
-        y, codes, exps, invstd = _bn8_forward(z.detach().contiguous(), w, b, rm, rv, eps, slope, batch_stats,
-                                              factor, col_sums)
-        out, sums = _product(y, weight, bias, want_sums)
-        if sums is None:
-            sums = torch.empty(0, dtype=torch.float64, device=z.device)
+        z = z.detach().contiguous()
+        ctx.fused = _fused8(z, weight)
+        if ctx.fused:
+            out, codes, exps, invstd, sums = _bn_linear8_forward(
+                z, w, b, rm, rv, eps, slope, batch_stats, factor, col_sums, weight, bias, want_sums)
+        else:
+            y, codes, exps, invstd = _bn8_forward(z, w, b, rm, rv, eps, slope, batch_stats, factor, col_sums)
+            out, sums = _product(y, weight, bias, want_sums)
         ctx.save_for_backward(codes, exps, w, b, invstd, weight)
         ctx.slope, ctx.batch_stats = slope, bool(batch_stats)
+        if sums is None:
+            return out, None
         ctx.mark_non_differentiable(sums)
         return out, sums
 
@@ -210,6 +294,9 @@ class _BatchNormActLinear8(torch.autograd.Function):
         need = ctx.needs_input_grad
         grad_out = grad_out.contiguous()
         gz = gw = gb = glw = glb = None
+        if ctx.fused and need[0] and need[3] and grad_out.data_ptr() % 16 == 0:
+            return _bn_linear8_backward(grad_out, codes, exps, w, b, invstd, ctx.batch_stats, ctx.slope, weight,
+                                        need) + (None,) * 8
         if any(need[:3]):
             gy = _product(grad_out, weight.t(), None)[0]
             gz, gw, gb = _bn8_backward(gy, codes, exps, w, b, invstd, ctx.batch_stats, ctx.slope, need)
@@ -278,7 +365,7 @@ def batch_norm_act_linear(z, bn, act, lin, col_sums=None, want_sums=False, keep=
             y, sums = _BatchNormActLinear8.apply(
                 z, bn.weight, bn.bias, lin.weight, lin.bias, rm, rv, bn.eps, float(act.negative_slope),
                 batch_stats, factor, col_sums if batch_stats else None, bool(want_sums))
-            return (y, sums if sums.numel() else None) if want_sums else y
+            return (y, sums) if want_sums else y
     return linear(lin, batch_norm_act(z, bn, act, col_sums=col_sums, keep=keep), want_sums, keep=keep)
 
 
@@ -400,12 +487,17 @@ class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, want_sums):
         codes = exps = None
-        if ctx.needs_input_grad[1]:
-            codes, exps = packed.pack_codes(x.detach().contiguous())
+        x = x.detach().contiguous()
+        ctx.fused = ctx.needs_input_grad[1] and _fused8(x, weight)
+        if ctx.fused:
+            y, codes, exps, sums = _linear8_forward(x, weight, bias, want_sums)
+        else:
+            if ctx.needs_input_grad[1]:
+                codes, exps = packed.pack_codes(x)
+            y, sums = _product(x, weight, bias, want_sums)
         ctx.save_for_backward(codes, exps, weight)
-        y, sums = _product(x, weight, bias, want_sums)
         if sums is None:
-            sums = torch.empty(0, dtype=torch.float64, device=x.device)
+            return y, None
         ctx.mark_non_differentiable(sums)
         return y, sums
 
@@ -415,6 +507,8 @@ class _Linear8(torch.autograd.Function):
         codes, exps, weight = ctx.saved_tensors
         need = ctx.needs_input_grad
         grad_y = grad_y.contiguous()
+        if ctx.fused and need[0] and grad_y.data_ptr() % 16 == 0:
+            return _linear8_backward(grad_y, codes, exps, weight, need[2]) + (None,)
         gx = _product(grad_y, weight.t(), None)[0] if need[0] else None
         gw = gb = None
         if need[1]:
@@ -442,7 +536,7 @@ def linear(lin, x, want_sums=False, keep=None):
     weight gradient, 'int8' its 8-bit rows; None: as ``keep_activations`` says."""
     if _takes(lin, x):
         y, sums = _linear(x, lin.weight, lin.bias, want_sums, keep)
-        return (y, sums if sums.numel() else None) if want_sums else y
+        return (y, sums if sums is not None and sums.numel() else None) if want_sums else y
     kept_form(keep)
     return (lin(x), None) if want_sums else lin(x)
 

@@ -264,16 +264,25 @@ def test_batch_norm_act_not_finite_rows():
 
 # ---- Linear and the block ------------------------------------------------------------------------
 def xty_bound(a, b, rows):
-    """Bound of sum |a||b| roundings of the kernel: per wave and step of 16 rows up to six matrix
+    """Bound of sum |a||b| roundings of the kernels: per wave and step of 16 rows up to six matrix
     instructions, each one rounding of the running sum and about 16 inside; a workgroup of four waves
-    has at least 256 rows, so a wave takes at most ceil(rows / (16 * 4 * workgroups)) + 1 steps."""
-    wgs = min(512, -(-rows // 256))
+    has at least 128 rows (256 workgroups at most), so a wave takes at most
+    ceil(rows / (16 * 4 * workgroups)) + 1 steps."""
+    wgs = min(256, -(-rows // 256))
     steps = -(-rows // (64 * wgs)) + 1
     return (6 * steps + 16 + 4) * U * (np.abs(a).T @ np.abs(b))
 
 
+def same_kernel(lin, y8, y32):
+    """From 4096 rows on both forms run the same product where mvf_linear_rows takes the shape."""
+    from mvfusion import _lib
+    if y8.shape[0] >= 4096 and _lib.load().mvf_linear_rows_supported(lin.in_features, lin.out_features):
+        assert torch.equal(y8, y32)
+
+
 @pytest.mark.parametrize("bias", [True, False])
-@pytest.mark.parametrize("rows,I,O", [(1, 8, 4), (15, 5, 3), (16, 32, 32), (33, 64, 64), (257, 40, 48), (1000, 33, 65),
+@pytest.mark.parametrize("rows,I,O", [(1, 8, 8), (31, 64, 64), (33, 16, 24), (4097, 64, 64), (40001, 32, 32), (5000, 8, 40),
+                                      (4128, 64, 8), (1, 8, 4), (15, 5, 3), (16, 32, 32), (33, 64, 64), (257, 40, 48), (1000, 33, 65),
                                       (4099, 64, 32), (9000, 7, 63), (5000, 50, 34), (700, 200, 130)])
 def test_linear(rows, I, O, bias):
     from mvfusion import training as tr
@@ -285,11 +294,12 @@ def test_linear(rows, I, O, bias):
     leaves = [xt, lin.weight] + ([lin.bias] if bias else [])
     y = tr.linear(lin, xt, keep="int8")
     grads = torch.autograd.grad(y, leaves, T(gy).cuda())
-    y32 = tr.linear(lin, xt, keep="float32")
-    g32 = torch.autograd.grad(y32, leaves, T(gy).cuda())
-    assert torch.equal(y, y32) and torch.equal(grads[0], g32[0])
+    same_kernel(lin, y, tr.linear(lin, xt, keep="float32"))
     xq = ref.unpack(*ref.pack(x))
-    g64 = gy.astype(np.float64)
+    g64, x64, w64 = gy.astype(np.float64), x.astype(np.float64), lin.weight.detach().cpu().double().numpy()
+    b64 = lin.bias.detach().cpu().double().numpy() if bias else np.zeros(O)
+    within(y.detach().cpu().numpy(), x64 @ w64.T + b64, (I + 2) * U * (np.abs(x64) @ np.abs(w64).T + np.abs(b64)), "y")
+    within(grads[0].cpu().numpy(), g64 @ w64, (O + 2) * U * (np.abs(g64) @ np.abs(w64)), "x")
     within(grads[1].cpu().numpy(), g64.T @ xq, xty_bound(g64, xq, rows), "weight")
     if bias:
         steps = -(-rows // 64) + 12
@@ -340,7 +350,8 @@ def test_linear_gradient_magnitudes():
 
 @pytest.mark.parametrize("training", [True, False])
 @pytest.mark.parametrize("rows,I,O,bias", [(16, 8, 4, False), (250, 33, 20, True), (1031, 64, 64, False), (5003, 32, 48, True),
-                                           (4500, 16, 33, False), (600, 100, 70, True)])
+                                           (31, 64, 8, True), (4096, 8, 16, False), (4129, 64, 64, True), (30011, 32, 32, False),
+                                           (65, 16, 40, True), (4500, 16, 33, False), (600, 100, 70, True)])
 def test_block(rows, I, O, bias, training):
     """BatchNorm + LeakyReLU + Linear from one packed copy of the normalised rows."""
     from mvfusion import training as tr
@@ -357,10 +368,19 @@ def test_block(rows, I, O, bias, training):
     after = {k: v.clone() for k, v in bn.state_dict().items()}
     bn.load_state_dict(before)
     y = tr.batch_norm_act_linear(zt, bn, act, lin, keep="int8")
-    assert torch.equal(y, y32) and all(torch.equal(v, after[k]) for k, v in bn.state_dict().items())
+    same_kernel(lin, y, y32)
+    assert all(torch.equal(v, after[k]) for k, v in bn.state_dict().items())
     leaves = [zt, bn.weight, bn.bias, lin.weight] + ([lin.bias] if bias else [])
     grads = [t.cpu().numpy() for t in torch.autograd.grad(y, leaves, T(go).cuda())]
     go64, w = go.astype(np.float64), lin.weight.detach().cpu().double().numpy()
+    zh = (z.astype(np.float64) - (ref.bn_stats(z.astype(np.float64), bn.eps)[0] if training
+                                  else bn.running_mean.cpu().double().numpy())) * invstd
+    a = zh * gamma + beta
+    act64 = np.where(a > 0, a, slope * a)
+    # four roundings of the normalised value (its mean and spread among them), then the product's
+    mag = (np.abs(zh) + np.abs(z - zh / invstd) * invstd + np.abs(z) * invstd) * np.abs(gamma) + np.abs(beta)
+    b64 = lin.bias.detach().cpu().double().numpy() if bias else np.zeros(O)
+    within(y.detach().cpu().numpy(), act64 @ w.T + b64, (I + 8) * U * (mag @ np.abs(w).T + np.abs(b64)), "y")
     gy = go64 @ w
     err = (O + 2) * U * (np.abs(go64) @ np.abs(w))
     gz, bound, dw, e_dw, db, e_db = bn_backward_reference(gy, err, zq, on, gamma, invstd, True, slope, training)
@@ -415,7 +435,7 @@ def make_pool(seed=0):
     return QKVBimodalCSRPool(in_main=24, in_map=8, in_mod=64, nc_qk=8, num_groups=4).cuda().train()
 
 
-def pool_inputs(points=900, seed=1):
+def pool_inputs(points=6000, seed=1):
     g = np.random.default_rng(seed)
     sizes = g.poisson(4, points)
     sizes[g.random(points) < 0.2] = 0
