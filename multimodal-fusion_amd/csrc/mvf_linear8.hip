@@ -26,11 +26,15 @@
 
 namespace mvf {
 
-constexpr int L8_THREADS = 512;
-constexpr int L8_WAVES = L8_THREADS / 64;
+#ifndef L8F
+#define L8F 512
+#define L8A 512
+#endif
+constexpr int L8_FWD_THREADS = L8F;
+// (two waves per SIMD for 64 -> 64 columns, whose registers allow no third; three elsewhere)
+constexpr int l8_bwd_threads(int KO, int KI, int mode) { return KO <= 4 && KI <= 4 ? 768 : mode == 2 ? L8A : 512; }
 constexpr int L8_ROWS = 32;                 // rows per tile
 constexpr int L8_MAX_WGS = 256;             // one per compute unit
-constexpr int L8_SUMS_ROWS = 1024;          // partial rows of column sums that mvf_linear_rows_sums_bytes has room for
 
 typedef float l8_f4 __attribute__((ext_vector_type(4)));
 typedef float l8_f2 __attribute__((ext_vector_type(2)));
@@ -75,14 +79,14 @@ template <int IQ> __device__ __forceinline__ unsigned l8_group_max(unsigned v)
 // ---- forward ----------------------------------------------------------------------------------
 // EXACT: O = 32 NO columns out, a constant.
 template <int KQ, int NO, bool TAIL, bool STATS, bool EXACT>
-__global__ __launch_bounds__(L8_THREADS) void linear8_forward_kernel(
-    const float *__restrict__ x, const float *__restrict__ W, const float *__restrict__ bias, int O_, i64 rows,
-    L8Bn bn, float *__restrict__ y, int8_t *__restrict__ codes, uint8_t *__restrict__ exps, double *__restrict__ col_sums)
+__global__ __launch_bounds__(L8_FWD_THREADS) void linear8_forward_kernel(
+    const float *x, const float *W, const float *bias, int O_, i64 rows,
+    L8Bn bn, float *y, int8_t *codes, uint8_t *exps, double *col_sums)
 {
     constexpr int I = 8 * KQ, IQ = 2 * KQ, HALF = 4 * KQ, GR = I > 32 ? 2 : 1;
     const int O = EXACT ? 32 * NO : O_;
-    constexpr int PITCH_I = I * 4 + 16;
-    __shared__ __attribute__((aligned(16))) char lds[L8_WAVES][L8_ROWS * (64 * 4 + 16)];
+    constexpr int PITCH_I = I * 4 + 16, THREADS = L8_FWD_THREADS, WAVES = THREADS / 64;
+    __shared__ __attribute__((aligned(16))) char lds[WAVES][L8_ROWS * (64 * 4 + 16)];
     __shared__ __attribute__((aligned(16))) char wlds[32 * NO * PITCH_I];
     __shared__ __attribute__((aligned(16))) float blds[32 * NO];
     // BatchNorm's terms of the columns: float64 mean and 1 / spread; the same in float32, weight, bias;
@@ -96,7 +100,7 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_forward_kernel(
     char *buf = lds[wave];
 
     // W as rows (zeros past O): the first operand, lane = output channel, k = the lane half's columns
-    for (int i = threadIdx.x; i < 32 * NO * I; i += L8_THREADS)
+    for (int i = threadIdx.x; i < 32 * NO * I; i += THREADS)
         *(float *)(wlds + i / I * PITCH_I + i % I * 4) = i / I < O ? W[i] : 0.0f;
     if (threadIdx.x < 32 * NO) blds[threadIdx.x] = bias && (int)threadIdx.x < O ? bias[threadIdx.x] : 0.0f;
     if constexpr (TAIL) {
@@ -127,7 +131,7 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_forward_kernel(
     const int col = 4 * (lane % IQ), row0 = lane / IQ;
     const i64 nfull = rows / L8_ROWS;       // whole tiles; the rows behind them are a tile of their own
     const int rest = (int)(rows - nfull * L8_ROWS);
-    const i64 wid = (i64)blockIdx.x * L8_WAVES + wave, nwaves = (i64)gridDim.x * L8_WAVES;
+    const i64 wid = (i64)blockIdx.x * WAVES + wave, nwaves = (i64)gridDim.x * WAVES;
     l8_f4 g[KQ];
     auto load_tile = [&](i64 t, int live) {
         const l8_f4 *src = (const l8_f4 *)(x + (size_t)t * L8_ROWS * I);
@@ -202,7 +206,10 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_forward_kernel(
             const l8_f4 p = {v[0], v[1], v[2], v[3]};
             *(l8_f4 *)(buf + r * PITCH_I + col * 4) = p;
         }
+        // (fenced: left alone, the scheduler moves the loads down to their use)
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (decltype(how)::NEXT) load_tile(next, L8_ROWS);
+        __builtin_amdgcn_sched_barrier(0);
         l8_wave_sync();
         float xv[4 * KQ];
 #pragma unroll
@@ -265,7 +272,11 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_forward_kernel(
     if (wid < nfull) {
         load_tile(wid, L8_ROWS);
         // (the last tile asks for itself once more, rather than for nothing under a condition)
-        for (i64 t = wid; t < nfull; t += nwaves) tile(t, L8_ROWS, t + nwaves < nfull ? t + nwaves : t, L8Tile<EXACT, true>());
+        // (and the first tile outside the loop: with its stores behind the loads of the second, the loop is
+        // entered as it is repeated, and its waits need not allow for fewer)
+        i64 t = wid;
+        tile(t, L8_ROWS, t + nwaves < nfull ? t + nwaves : t, L8Tile<EXACT, true>());
+        for (t += nwaves; t < nfull; t += nwaves) tile(t, L8_ROWS, t + nwaves < nfull ? t + nwaves : t, L8Tile<EXACT, true>());
     }
     if (rest > 0 && wid == nfull % nwaves) {
         load_tile(nfull, rest);
@@ -276,10 +287,18 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_forward_kernel(
             sum1 += __shfl_xor(sum1, 32, 64);
             sum2 += __shfl_xor(sum2, 32, 64);
         }
-        double *out = col_sums + (size_t)wid * 2 * O;
+        // the workgroup's waves in order
+        __syncthreads();
+        double *red = (double *)lds[0];
         if (lane < 32 * NO && sc < O) {
-            out[sc] = sum1;
-            out[O + sc] = sum2;
+            red[wave * 2 * O + sc] = sum1;
+            red[wave * 2 * O + O + sc] = sum2;
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < 2 * O) {
+            double t = red[threadIdx.x];
+            for (int k = 1; k < WAVES; ++k) t += red[k * 2 * O + threadIdx.x];
+            col_sums[(size_t)blockIdx.x * 2 * O + threadIdx.x] = t;
         }
     }
 }
@@ -289,12 +308,13 @@ enum { L8_LINEAR = 0, L8_SUMS = 1, L8_APPLY = 2 };
 
 // O <= 8 KO columns of g (EXACT: 8 KO, a constant), I = 8 KI columns of the kept rows.
 template <int KO, int KI, int MODE, bool EXACT>
-__global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
-    const float *__restrict__ gsrc, int O_, const int8_t *__restrict__ codes, const uint8_t *__restrict__ exps,
-    const float *__restrict__ W, i64 rows, L8Bn bn, int want_sums, float *__restrict__ grad,
-    float *__restrict__ partial, float *__restrict__ partial_sums, double *__restrict__ partial_bn)
+__global__ __launch_bounds__(l8_bwd_threads(KO, KI, MODE)) void linear8_backward_kernel(
+    const float *gsrc, int O_, const int8_t *codes, const uint8_t *exps,
+    const float *W, i64 rows, L8Bn bn, int want_sums, float *grad,
+    float *partial, float *partial_sums, double *partial_bn)
 {
     constexpr int I = 8 * KI, IQ = 2 * KI, GR = I > 32 ? 2 : 1;
+    constexpr int THREADS = l8_bwd_threads(KO, KI, MODE), WAVES = THREADS / 64;
     const int O = EXACT ? 8 * KO : O_;
     constexpr int NI = I > 32 ? 2 : 1, NA = KO > 4 ? 2 : 1;
     constexpr int PITCH_I = I * 4 + 16;
@@ -303,9 +323,9 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
     constexpr int PITCH_Q = I * 2 + 16, PLANE = L8_ROWS * PITCH_Q;
     constexpr int TILE = L8_ROWS * ((KO * 8 > I ? KO * 8 : I) * 4 + 16);
     constexpr int REGION = TILE + (XTY ? PLANE : 0);
-    constexpr int FOLD = XTY ? (NA * NI * 1024 + L8_WAVES * 64) * 4 : 0;
-    constexpr int RED = MODE == L8_SUMS ? L8_WAVES * 2 * I * 8 : 0;
-    constexpr int LDS = L8_WAVES * REGION > FOLD + RED ? L8_WAVES * REGION : FOLD + RED;
+    constexpr int FOLD = XTY ? (NA * NI * 1024 + WAVES * 64) * 4 : 0;
+    constexpr int RED = MODE == L8_SUMS ? WAVES * 2 * I * 8 : 0;
+    constexpr int LDS = WAVES * REGION > FOLD + RED ? WAVES * REGION : FOLD + RED;
     __shared__ __attribute__((aligned(16))) char lds[LDS];
     __shared__ __attribute__((aligned(16))) char wlds[32 * NI * PITCH_W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -316,7 +336,7 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
 
     // W transposed (zeros past I, and past O): the product's first operand, lane = column of the kept
     // rows, k = the lane half's columns of g
-    for (int i = threadIdx.x; i < 32 * NI * KO * 8; i += L8_THREADS) {
+    for (int i = threadIdx.x; i < 32 * NI * KO * 8; i += THREADS) {
         const int c = i % (32 * NI), o = i / (32 * NI);
         *(float *)(wlds + c * PITCH_W + o * 4) = c < I && o < O ? W[(size_t)o * I + c] : 0.0f;
     }
@@ -376,7 +396,7 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
 
     const i64 nfull = rows / L8_ROWS;
     const int rest = (int)(rows - nfull * L8_ROWS);
-    const i64 wid = (i64)blockIdx.x * L8_WAVES + wave, nwaves = (i64)gridDim.x * L8_WAVES;
+    const i64 wid = (i64)blockIdx.x * WAVES + wave, nwaves = (i64)gridDim.x * WAVES;
     l8_f4 g[KO];
     unsigned qw[KI];
     int ew;
@@ -497,8 +517,9 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
         }
         // the next tile asked for here, where the weight gradient's operands have left their registers; the
         // product hides its way
-        if constexpr (XTY) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (decltype(how)::NEXT) load_tile(next, L8_ROWS);
+        __builtin_amdgcn_sched_barrier(0);
         // g W: lane = row
         xty_acc acc[NI];
 #pragma unroll
@@ -574,7 +595,9 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
     };
     if (wid < nfull) {
         load_tile(wid, L8_ROWS);
-        for (i64 t = wid; t < nfull; t += nwaves) tile(t, L8_ROWS, t + nwaves < nfull ? t + nwaves : t, L8Tile<true, true>());
+        i64 t = wid;
+        tile(t, L8_ROWS, t + nwaves < nfull ? t + nwaves : t, L8Tile<true, true>());
+        for (t += nwaves; t < nfull; t += nwaves) tile(t, L8_ROWS, t + nwaves < nfull ? t + nwaves : t, L8Tile<true, true>());
     }
     if (rest > 0 && wid == nfull % nwaves) {
         load_tile(nfull, rest);
@@ -584,7 +607,7 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
     if constexpr (XTY) {
         __syncthreads();
         float *fold = (float *)lds, *fold_sums = fold + NA * NI * 1024;
-        for (int turn = 0; turn < L8_WAVES; ++turn) {
+        for (int turn = 0; turn < WAVES; ++turn) {
             if (wave == turn) {
 #pragma unroll
                 for (int i = 0; i < NA; ++i)
@@ -599,7 +622,7 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
             __syncthreads();
         }
         float *p = partial + (size_t)blockIdx.x * (NA * NI * 1024);
-        for (int at = threadIdx.x; at < NA * NI * 1024; at += L8_THREADS) p[at] = fold[at];
+        for (int at = threadIdx.x; at < NA * NI * 1024; at += THREADS) p[at] = fold[at];
         if (want_sums) {
 #pragma unroll
             for (int i = 0; i < NA; ++i) {
@@ -610,7 +633,7 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
             if (threadIdx.x < 32 * NA) {
                 float s = 0.0f;
 #pragma unroll
-                for (int k = 0; k < L8_WAVES; ++k) s += fold_sums[k * 64 + threadIdx.x];
+                for (int k = 0; k < WAVES; ++k) s += fold_sums[k * 64 + threadIdx.x];
                 partial_sums[(size_t)blockIdx.x * 64 + threadIdx.x] = s;
             }
         }
@@ -631,23 +654,24 @@ __global__ __launch_bounds__(L8_THREADS) void linear8_backward_kernel(
                 red[(wave * 2 + 1) * I + col + k] = bq[k];
             }
         __syncthreads();
-        for (int c = threadIdx.x; c < 2 * I; c += L8_THREADS) {
+        for (int c = threadIdx.x; c < 2 * I; c += THREADS) {
             double s = red[c];
-            for (int k = 1; k < L8_WAVES; ++k) s += red[k * 2 * I + c];
+            for (int k = 1; k < WAVES; ++k) s += red[k * 2 * I + c];
             partial_bn[(size_t)blockIdx.x * 2 * I + c] = s;
         }
     }
 }
 
-static int l8_workgroups(i64 rows, int most = L8_MAX_WGS)
+static int l8_workgroups(i64 rows, int threads)
 {
     int dev = 0, cus = 256;
     if (hipGetDevice(&dev) != hipSuccess ||
         hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) cus = 256;
     const i64 ntiles = (rows + L8_ROWS - 1) / L8_ROWS;
-    i64 n = (ntiles + L8_WAVES - 1) / L8_WAVES;
+    const int waves = threads / 64;
+    i64 n = (ntiles + waves - 1) / waves;
     if (n > cus) n = cus;
-    if (n > most) n = most;
+    if (n > L8_MAX_WGS) n = L8_MAX_WGS;
     return (int)n;
 }
 
@@ -659,10 +683,10 @@ static void l8_forward(const float *x, int I, const float *W, const float *bias,
 #define MVF_L8F(KQ_, NO_, ST_)                                                                                     \
     do {                                                                                                           \
         if (O == 32 * NO_)                                                                                         \
-            hipLaunchKernelGGL((linear8_forward_kernel<KQ_, NO_, TAIL, ST_, true>), dim3((unsigned)nwg), dim3(L8_THREADS), 0, \
+            hipLaunchKernelGGL((linear8_forward_kernel<KQ_, NO_, TAIL, ST_, true>), dim3((unsigned)nwg), dim3(L8_FWD_THREADS), 0, \
                                st, x, W, bias, O, rows, bn, y, codes, exps, col_sums);                             \
         else                                                                                                       \
-            hipLaunchKernelGGL((linear8_forward_kernel<KQ_, NO_, TAIL, ST_, false>), dim3((unsigned)nwg), dim3(L8_THREADS), 0, \
+            hipLaunchKernelGGL((linear8_forward_kernel<KQ_, NO_, TAIL, ST_, false>), dim3((unsigned)nwg), dim3(L8_FWD_THREADS), 0, \
                                st, x, W, bias, O, rows, bn, y, codes, exps, col_sums);                             \
     } while (0)
 #define MVF_L8F_NO(KQ_)                                                                                            \
@@ -677,18 +701,22 @@ static void l8_forward(const float *x, int I, const float *W, const float *bias,
 #undef MVF_L8F
 }
 
+// (the workgroups launched: the partial results there are)
 template <int MODE>
-static void l8_backward(const float *g, int O, const int8_t *codes, const uint8_t *exps, const float *W, int I, i64 rows,
+static int l8_backward(const float *g, int O, const int8_t *codes, const uint8_t *exps, const float *W, int I, i64 rows,
                         const L8Bn &bn, int want_sums, float *grad, float *partial, float *partial_sums, double *partial_bn,
-                        int nwg, hipStream_t st)
+                        hipStream_t st)
 {
+    int nwg = 0;
 #define MVF_L8B(KO_, KI_)                                                                                          \
     do {                                                                                                           \
+        constexpr int threads = l8_bwd_threads(KO_, KI_, MODE);                                                    \
+        nwg = l8_workgroups(rows, threads);                                                                        \
         if (O == 8 * KO_)                                                                                          \
-            hipLaunchKernelGGL((linear8_backward_kernel<KO_, KI_, MODE, true>), dim3((unsigned)nwg), dim3(L8_THREADS), 0, st, \
+            hipLaunchKernelGGL((linear8_backward_kernel<KO_, KI_, MODE, true>), dim3((unsigned)nwg), dim3(threads), 0, st, \
                                g, O, codes, exps, W, rows, bn, want_sums, grad, partial, partial_sums, partial_bn); \
         else                                                                                                       \
-            hipLaunchKernelGGL((linear8_backward_kernel<KO_, KI_, MODE, false>), dim3((unsigned)nwg), dim3(L8_THREADS), 0, st, \
+            hipLaunchKernelGGL((linear8_backward_kernel<KO_, KI_, MODE, false>), dim3((unsigned)nwg), dim3(threads), 0, st, \
                                g, O, codes, exps, W, rows, bn, want_sums, grad, partial, partial_sums, partial_bn); \
     } while (0)
 #define MVF_L8B_KI(KO_)                                                                                            \
@@ -706,6 +734,7 @@ static void l8_backward(const float *g, int O, const int8_t *codes, const uint8_
     else MVF_L8B_KI(8);
 #undef MVF_L8B_KI
 #undef MVF_L8B
+    return nwg;
 }
 
 // fold of linear8_backward_kernel's weight-gradient partials
@@ -736,8 +765,8 @@ extern "C" int mvf_linear_rows8_forward(
     MVF_REQUIRE(l8_aligned(x, 16) && l8_aligned(y, 16) && l8_aligned(codes, 4), "linear_rows8_forward: x, y or codes not aligned");
     MVF_REQUIRE(!col_sums || (n_col_sums && col_sums_bytes >= mvf_linear_rows_sums_bytes(O)),
                 "linear_rows8_forward: too small buffer for the column sums");
-    const int nwg = l8_workgroups(rows, col_sums ? L8_SUMS_ROWS / L8_WAVES : L8_MAX_WGS);
-    if (n_col_sums) *n_col_sums = col_sums ? nwg * L8_WAVES : 0;
+    const int nwg = l8_workgroups(rows, L8_FWD_THREADS);
+    if (n_col_sums) *n_col_sums = col_sums ? nwg : 0;
     l8_forward<false>(x, I, weight, bias, O, rows, L8Bn{}, y, codes, exps, col_sums, nwg, (hipStream_t)stream);
     MVF_LAUNCH_CHECK();
     return MVF_OK;
@@ -755,9 +784,8 @@ extern "C" int mvf_linear_rows8_backward(
     MVF_REQUIRE(workspace && workspace_bytes >= mvf_xty8_workspace_bytes(), "linear_rows8_backward: workspace too small");
     hipStream_t st = (hipStream_t)stream;
     float *partial = (float *)workspace, *partial_sums = (float *)((char *)workspace + mvf_xty_workspace_bytes());
-    const int nwg = l8_workgroups(rows);
-    l8_backward<L8_LINEAR>(grad_y, O, codes, exps, weight, I, rows, L8Bn{}, grad_bias != nullptr, grad_x, partial, partial_sums,
-                           nullptr, nwg, st);
+    const int nwg = l8_backward<L8_LINEAR>(grad_y, O, codes, exps, weight, I, rows, L8Bn{}, grad_bias != nullptr, grad_x, partial,
+                                           partial_sums, nullptr, st);
     l8_fold(partial, partial_sums, nwg, I, O, grad_weight, grad_bias, st);
     MVF_LAUNCH_CHECK();
     return MVF_OK;
@@ -790,8 +818,8 @@ extern "C" int mvf_batch_norm_act_linear8_forward(
     const Bn8Workspace w = bn8_workspace(workspace, I);
     bn8_statistics(z, rows, I, running_mean, running_var, training, momentum, eps, col_sums, n_col_sums, w, save_invstd, st);
     const L8Bn bn = {w.terms, save_invstd, w.terms64, bn_weight, bn_bias, nullptr, act, training, slope};
-    const int nwg = l8_workgroups(rows, y_sums ? L8_SUMS_ROWS / L8_WAVES : L8_MAX_WGS);
-    if (n_y_sums) *n_y_sums = y_sums ? nwg * L8_WAVES : 0;
+    const int nwg = l8_workgroups(rows, L8_FWD_THREADS);
+    if (n_y_sums) *n_y_sums = y_sums ? nwg : 0;
     l8_forward<true>(z, I, weight, bias, O, rows, bn, y, codes, exps, y_sums, nwg, st);
     MVF_LAUNCH_CHECK();
     return MVF_OK;
@@ -815,13 +843,12 @@ extern "C" int mvf_batch_norm_act_linear8_backward(
     char *xty = (char *)workspace + mvf_batch_norm_act8_workspace_bytes(I);
     float *partial = (float *)xty, *partial_sums = (float *)(xty + mvf_xty_workspace_bytes());
     const L8Bn bn = {nullptr, save_invstd, nullptr, bn_weight, bn_bias, w.terms, act, training, act ? slope : 1.0f};
-    const int nwg = l8_workgroups(rows);
-    l8_backward<L8_SUMS>(grad_y, O, codes, exps, weight, I, rows, bn, grad_bias != nullptr, nullptr, partial, partial_sums,
-                         w.partial, nwg, st);
+    const int nwg = l8_backward<L8_SUMS>(grad_y, O, codes, exps, weight, I, rows, bn, grad_bias != nullptr, nullptr, partial,
+                                         partial_sums, w.partial, st);
     l8_fold(partial, partial_sums, nwg, I, O, grad_weight, grad_bias, st);
     bn8_grad_terms(w, nwg, I, rows, grad_bn_weight, grad_bn_bias, st);
     if (grad_z)
-        l8_backward<L8_APPLY>(grad_y, O, codes, exps, weight, I, rows, bn, 0, grad_z, nullptr, nullptr, nullptr, nwg, st);
+        l8_backward<L8_APPLY>(grad_y, O, codes, exps, weight, I, rows, bn, 0, grad_z, nullptr, nullptr, nullptr, st);
     MVF_LAUNCH_CHECK();
     return MVF_OK;
 }
