@@ -518,6 +518,7 @@ int mvf_unpack_rows8(
  * be NULL), codes / exps of zhat (computed in float64), save_invstd [C].  With an
  * activation a code reads back on the side of the kink -beta / gamma (rounded
  * to float32) on which the value lies: it is moved by at most one step for that.
+ * num_batches (may be NULL): a counter that training adds 1 to.
  * backward: the formulas of mvf_batch_norm_act_backward with zhat as read back
  * and the activation's side taken from it; grad_z, grad_weight, grad_bias may be
  * NULL.  weight and bias are the ones of the forward.  workspace:
@@ -526,7 +527,7 @@ size_t mvf_batch_norm_act8_workspace_bytes(int32_t C);
 int mvf_batch_norm_act8_forward(
     const float *z, int64_t rows, int32_t C, const float *weight, const float *bias,
     float *running_mean, float *running_var, int32_t training, float momentum, float eps,
-    int32_t act, float slope, float *y, int8_t *codes, uint8_t *exps, float *save_invstd,
+    int32_t act, float slope, int64_t *num_batches, float *y, int8_t *codes, uint8_t *exps, float *save_invstd,
     const double *col_sums, int32_t n_col_sums, void *workspace, size_t workspace_bytes, void *stream);
 int mvf_batch_norm_act8_backward(
     const float *grad_y, const int8_t *codes, const uint8_t *exps, int64_t rows, int32_t C,
@@ -573,7 +574,7 @@ size_t mvf_batch_norm_act_linear8_workspace_bytes(int32_t I);
 int mvf_batch_norm_act_linear8_forward(
     const float *z, int64_t rows, int32_t I, const float *bn_weight, const float *bn_bias,
     float *running_mean, float *running_var, int32_t training, float momentum, float eps, int32_t act, float slope,
-    const float *weight, const float *bias, int32_t O, float *y, int8_t *codes, uint8_t *exps, float *save_invstd,
+    int64_t *num_batches, const float *weight, const float *bias, int32_t O, float *y, int8_t *codes, uint8_t *exps, float *save_invstd,
     const double *col_sums, int32_t n_col_sums, double *y_sums, size_t y_sums_bytes, int32_t *n_y_sums,
     void *workspace, size_t workspace_bytes, void *stream);
 int mvf_batch_norm_act_linear8_backward(

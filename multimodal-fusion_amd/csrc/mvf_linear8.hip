@@ -254,7 +254,7 @@ __global__ __launch_bounds__(L8_FWD_THREADS) void linear8_forward_kernel(
 #pragma unroll
         for (int j = 0; j < 4 * NO; ++j) {
             const int f = lane + 64 * j;
-            if (WHOLE || f < live * oq) dst[f] = *(const l8_f4 *)(buf + out_at[j]);
+            if (WHOLE || f < live * oq) r8_stream(dst + f, *(const l8_f4 *)(buf + out_at[j]));
         }
         if constexpr (STATS) {
             if (sc < O) {
@@ -581,7 +581,7 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI, MODE)) void linear8_backward
                 }
             }
             if constexpr (MODE != L8_SUMS) {
-                if (WHOLE || r < live) dst[lane + 64 * j] = v;
+                if (WHOLE || r < live) r8_stream(dst + lane + 64 * j, v);
             }
         }
         if constexpr (MODE == L8_SUMS) {
@@ -799,7 +799,7 @@ extern "C" size_t mvf_batch_norm_act_linear8_workspace_bytes(int32_t I)
 extern "C" int mvf_batch_norm_act_linear8_forward(
     const float *z, int64_t rows, int32_t I, const float *bn_weight, const float *bn_bias,
     float *running_mean, float *running_var, int32_t training, float momentum, float eps, int32_t act, float slope,
-    const float *weight, const float *bias, int32_t O, float *y, int8_t *codes, uint8_t *exps, float *save_invstd,
+    int64_t *num_batches, const float *weight, const float *bias, int32_t O, float *y, int8_t *codes, uint8_t *exps, float *save_invstd,
     const double *col_sums, int32_t n_col_sums, double *y_sums, size_t y_sums_bytes, int32_t *n_y_sums,
     void *workspace, size_t workspace_bytes, void *stream)
 {
@@ -816,7 +816,8 @@ extern "C" int mvf_batch_norm_act_linear8_forward(
                 "batch_norm_act_linear8_forward: workspace too small");
     hipStream_t st = (hipStream_t)stream;
     const Bn8Workspace w = bn8_workspace(workspace, I);
-    bn8_statistics(z, rows, I, running_mean, running_var, training, momentum, eps, col_sums, n_col_sums, w, save_invstd, st);
+    bn8_statistics(z, rows, I, running_mean, running_var, training, momentum, eps, col_sums, n_col_sums, (long long *)num_batches, w,
+                   save_invstd, st);
     const L8Bn bn = {w.terms, save_invstd, w.terms64, bn_weight, bn_bias, nullptr, act, training, slope};
     const int nwg = l8_workgroups(rows, L8_FWD_THREADS);
     if (n_y_sums) *n_y_sums = y_sums ? nwg : 0;

@@ -17,9 +17,11 @@ struct Bn8Workspace {
 Bn8Workspace bn8_workspace(void *workspace, int C);
 
 // mean and invstd in float32 (terms, save_invstd) and float64 (terms64): of the batch, from col_sums if
-// given, with the running statistics updated; or of the running statistics.
+// given, with the running statistics updated and the batch counted in num_batches (may be NULL); or of
+// the running statistics.
 void bn8_statistics(const float *z, i64 rows, int C, float *running_mean, float *running_var, int training, float momentum,
-                    float eps, const double *col_sums, int n_col_sums, const Bn8Workspace &w, float *save_invstd, hipStream_t st);
+                    float eps, const double *col_sums, int n_col_sums, long long *num_batches, const Bn8Workspace &w,
+                    float *save_invstd, hipStream_t st);
 
 // gradients of weight and bias (may be NULL) and the column means, from nblk rows of w.partial
 void bn8_grad_terms(const Bn8Workspace &w, int nblk, int C, i64 rows, float *grad_weight, float *grad_bias, hipStream_t st);

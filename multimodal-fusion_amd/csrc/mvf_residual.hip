@@ -176,7 +176,7 @@ __device__ __forceinline__ void piece_store(typename R::T *row, int col, int C, 
     }
     if (VEC && col < C) {
         const r8_u4 t = {w[0], w[1], w[2], w[3]};
-        *reinterpret_cast<r8_u4 *>(row + col) = t;
+        r8_stream(reinterpret_cast<r8_u4 *>(row + col), t);
     } else if (!VEC && col + W <= C) {
         if constexpr (W == 4) {
             const R8Words4 t = {{w[0], w[1], w[2], w[3]}};

@@ -113,7 +113,7 @@ _SIGNATURES = {
     "mvf_pack_rows8": (C.c_int, [_P, _I32, _I64, _I32, _P, _P, _P]),
     "mvf_unpack_rows8": (C.c_int, [_P, _P, _I64, _I32, _P, _I32, _P]),
     "mvf_batch_norm_act8_workspace_bytes": (_SZ, [_I32]),
-    "mvf_batch_norm_act8_forward": (C.c_int, [_P, _I64, _I32, _P, _P, _P, _P, _I32, _F, _F, _I32, _F,
+    "mvf_batch_norm_act8_forward": (C.c_int, [_P, _I64, _I32, _P, _P, _P, _P, _I32, _F, _F, _I32, _F, _P,
                                               _P, _P, _P, _P, _P, _I32, _P, _SZ, _P]),
     "mvf_batch_norm_act8_backward": (C.c_int, [_P, _P, _P, _I64, _I32, _P, _P, _P, _I32, _I32, _F,
                                                _P, _P, _P, _P, _SZ, _P]),
@@ -124,7 +124,7 @@ _SIGNATURES = {
     "mvf_linear_rows8_forward": (C.c_int, [_P, _I32, _P, _P, _I32, _I64, _P, _P, _P, _P, _SZ, _P, _P]),
     "mvf_linear_rows8_backward": (C.c_int, [_P, _P, _P, _P, _I32, _I32, _I64, _P, _P, _P, _P, _SZ, _P]),
     "mvf_batch_norm_act_linear8_workspace_bytes": (_SZ, [_I32]),
-    "mvf_batch_norm_act_linear8_forward": (C.c_int, [_P, _I64, _I32, _P, _P, _P, _P, _I32, _F, _F, _I32, _F,
+    "mvf_batch_norm_act_linear8_forward": (C.c_int, [_P, _I64, _I32, _P, _P, _P, _P, _I32, _F, _F, _I32, _F, _P,
                                                      _P, _P, _I32, _P, _P, _P, _P, _P, _I32, _P, _SZ, _P,
                                                      _P, _SZ, _P]),
     "mvf_batch_norm_act_linear8_backward": (C.c_int, [_P, _P, _P, _I64, _I32, _P, _P, _P, _I32, _I32, _F, _P, _I32,

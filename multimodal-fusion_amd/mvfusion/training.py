@@ -128,7 +128,7 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _bn8_forward(z, weight, bias, rm, rv, eps, slope, batch_stats, factor, col_sums):
+def _bn8_forward(z, weight, bias, rm, rv, eps, slope, batch_stats, factor, counter, col_sums):
     """(y, codes, exps, invstd) of mvf_batch_norm_act8_forward."""
     lib = L.load()
     rows, C = z.shape
@@ -139,7 +139,7 @@ def _bn8_forward(z, weight, bias, rm, rv, eps, slope, batch_stats, factor, col_s
     nbytes = lib.mvf_batch_norm_act8_workspace_bytes(C)
     ws = L.workspace(nbytes, dev)
     L.launch(dev, lib.mvf_batch_norm_act8_forward, z.data_ptr(), rows, C, _addr(weight), _addr(bias), _addr(rm),
-             _addr(rv), batch_stats, factor, eps, slope is not None, slope or 0.0, y.data_ptr(), codes.data_ptr(),
+             _addr(rv), batch_stats, factor, eps, slope is not None, slope or 0.0, _addr(counter), y.data_ptr(), codes.data_ptr(),
              exps.data_ptr(), invstd.data_ptr(), _addr(col_sums), 0 if col_sums is None else col_sums.shape[0],
              ws.data_ptr(), nbytes)
     return y, codes, exps, invstd
@@ -204,7 +204,7 @@ def _linear8_backward(grad_y, codes, exps, weight, want_bias):
     return gx, gw, gb
 
 
-def _bn_linear8_forward(z, w, b, rm, rv, eps, slope, batch_stats, factor, col_sums, weight, bias, want_sums):
+def _bn_linear8_forward(z, w, b, rm, rv, eps, slope, batch_stats, factor, counter, col_sums, weight, bias, want_sums):
     """(out, codes, exps, invstd, partial column sums or None) of mvf_batch_norm_act_linear8_forward."""
     lib = L.load()
     rows, (cout, cin), dev = z.shape[0], weight.shape, z.device
@@ -216,7 +216,8 @@ def _bn_linear8_forward(z, w, b, rm, rv, eps, slope, batch_stats, factor, col_su
     nbytes = lib.mvf_batch_norm_act_linear8_workspace_bytes(cin)
     ws = L.workspace(nbytes, dev)
     L.launch(dev, lib.mvf_batch_norm_act_linear8_forward, z.data_ptr(), rows, cin, _addr(w), _addr(b), _addr(rm),
-             _addr(rv), batch_stats, factor, eps, slope is not None, slope or 0.0, weight.data_ptr(), _addr(bias), cout,
+             _addr(rv), batch_stats, factor, eps, slope is not None, slope or 0.0, _addr(counter), weight.data_ptr(),
+             _addr(bias), cout,
              out.data_ptr(), codes.data_ptr(), exps.data_ptr(), invstd.data_ptr(), _addr(col_sums),
              0 if col_sums is None else col_sums.shape[0], _addr(sums), sbytes, ctypes.addressof(n),
              ws.data_ptr(), nbytes)
@@ -248,10 +249,10 @@ class _BatchNormAct8(torch.autograd.Function):
     """_BatchNormAct that keeps the normalised rows in 8 bits."""
 
     @staticmethod
-    def forward(ctx, z, weight, bias, rm, rv, eps, slope, batch_stats, factor, col_sums):
+    def forward(ctx, z, weight, bias, rm, rv, eps, slope, batch_stats, factor, counter, col_sums):
         w, b = _vector(weight), _vector(bias)
         y, codes, exps, invstd = _bn8_forward(z.detach().contiguous(), w, b, rm, rv, eps, slope, batch_stats,
-                                              factor, col_sums)
+                                              factor, counter, col_sums)
         ctx.save_for_backward(codes, exps, w, b, invstd)
         ctx.slope, ctx.batch_stats = slope, bool(batch_stats)
         return y
@@ -261,7 +262,7 @@ class _BatchNormAct8(torch.autograd.Function):
     def backward(ctx, grad_y):
         codes, exps, w, b, invstd = ctx.saved_tensors
         return _bn8_backward(grad_y, codes, exps, w, b, invstd, ctx.batch_stats, ctx.slope,
-                             ctx.needs_input_grad) + (None,) * 7
+                             ctx.needs_input_grad) + (None,) * 8
 
 
 class _BatchNormActLinear8(torch.autograd.Function):
@@ -269,16 +270,16 @@ class _BatchNormActLinear8(torch.autograd.Function):
     a row: the Linear's input is made of them again in its weight gradient."""
 
     @staticmethod
-    def forward(ctx, z, bn_weight, bn_bias, weight, bias, rm, rv, eps, slope, batch_stats, factor, col_sums,
+    def forward(ctx, z, bn_weight, bn_bias, weight, bias, rm, rv, eps, slope, batch_stats, factor, counter, col_sums,
                 want_sums):
         w, b = _vector(bn_weight), _vector(bn_bias)
         z = z.detach().contiguous()
         ctx.fused = _fused8(z, weight)
         if ctx.fused:
             out, codes, exps, invstd, sums = _bn_linear8_forward(
-                z, w, b, rm, rv, eps, slope, batch_stats, factor, col_sums, weight, bias, want_sums)
+                z, w, b, rm, rv, eps, slope, batch_stats, factor, counter, col_sums, weight, bias, want_sums)
         else:
-            y, codes, exps, invstd = _bn8_forward(z, w, b, rm, rv, eps, slope, batch_stats, factor, col_sums)
+            y, codes, exps, invstd = _bn8_forward(z, w, b, rm, rv, eps, slope, batch_stats, factor, counter, col_sums)
             out, sums = _product(y, weight, bias, want_sums)
         ctx.save_for_backward(codes, exps, w, b, invstd, weight)
         ctx.slope, ctx.batch_stats = slope, bool(batch_stats)
@@ -296,7 +297,7 @@ class _BatchNormActLinear8(torch.autograd.Function):
         gz = gw = gb = glw = glb = None
         if ctx.fused and need[0] and need[3] and grad_out.data_ptr() % 16 == 0:
             return _bn_linear8_backward(grad_out, codes, exps, w, b, invstd, ctx.batch_stats, ctx.slope, weight,
-                                        need) + (None,) * 8
+                                        need) + (None,) * 9
         if any(need[:3]):
             gy = _product(grad_out, weight.t(), None)[0]
             gz, gw, gb = _bn8_backward(gy, codes, exps, w, b, invstd, ctx.batch_stats, ctx.slope, need)
@@ -304,31 +305,38 @@ class _BatchNormActLinear8(torch.autograd.Function):
             glw, glb = xty8(grad_out, codes, exps, tail=(w, b, ctx.slope), want_sums=need[4])
         elif need[4]:
             glb = xty(grad_out).view(-1)
-        return (gz, gw, gb, glw, glb) + (None,) * 8
+        return (gz, gw, gb, glw, glb) + (None,) * 9
 
 
-def _bn_plan(z, bn):
-    """(running mean, running variance, batch_stats, factor) of an nn.BatchNorm1d's next
-    call on z, its num_batches_tracked counted; None where this package's kernels do not
-    take z or the module."""
+def _bn_plan(z, bn, kernel_counts=False):
+    """(running mean, running variance, batch_stats, factor, counter) of an nn.BatchNorm1d's next
+    call on z; None where this package's kernels do not take z or the module.  The batch is
+    counted in num_batches_tracked here, or, with kernel_counts, by the kernel that is given
+    the counter (None: already counted, or nothing to count)."""
     if not (z.is_cuda and z.dtype == torch.float32 and z.dim() == 2 and z.shape[0] > 0
-            and isinstance(bn, torch.nn.BatchNorm1d)
-            and all(t is None or (t.is_cuda and t.dtype == torch.float32)
-                    for t in (bn.weight, bn.bias, bn.running_mean, bn.running_var))):
+            and isinstance(bn, torch.nn.BatchNorm1d)):
         return None
-    batch_stats = bn.training or bn.running_mean is None
-    factor = 0.0
+    weight, bias = bn._parameters["weight"], bn._parameters["bias"]
+    rm, rv, tracked = (bn._buffers.get(k) for k in ("running_mean", "running_var", "num_batches_tracked"))
+    for t in (weight, bias, rm, rv):
+        if t is not None and not (t.is_cuda and t.dtype == torch.float32):
+            return None
+    batch_stats = bn.training or rm is None
+    factor, counter = 0.0, None
     if batch_stats:
         if z.shape[0] < 2:
             raise ValueError(
                 f"Expected more than 1 value per channel when training, got input size {tuple(z.shape)}")
-        if bn.training and bn.track_running_stats and bn.num_batches_tracked is not None:
-            bn.num_batches_tracked.add_(1)
-            factor = (1.0 / float(bn.num_batches_tracked)) if bn.momentum is None else bn.momentum
+        if bn.training and bn.track_running_stats and tracked is not None:
+            if kernel_counts and bn.momentum is not None and tracked.is_cuda and tracked.dtype == torch.int64:
+                counter = tracked
+            else:
+                tracked.add_(1)
+            factor = (1.0 / float(tracked)) if bn.momentum is None else bn.momentum
     # running statistics: updated in train mode, read in eval mode, unused by an eval-mode
     # module that tracks none (it normalises with batch statistics)
-    use_running = bn.running_mean is not None and (bn.training or not batch_stats)
-    return (bn.running_mean if use_running else None, bn.running_var if use_running else None, batch_stats, factor)
+    use_running = rm is not None and (bn.training or not batch_stats)
+    return (rm if use_running else None, rv if use_running else None, batch_stats, factor, counter)
 
 
 def batch_norm_act(z, bn, act, col_sums=None, keep=None):
@@ -343,13 +351,16 @@ def batch_norm_act(z, bn, act, col_sums=None, keep=None):
     None: as ``keep_activations`` says."""
     fused_act = isinstance(act, torch.nn.LeakyReLU)
     keeps8 = _keeps8(keep, z, bn.weight, bn.bias)
-    plan = _bn_plan(z, bn)
+    plan = _bn_plan(z, bn, keeps8)
     if plan is None:
         return act(bn(z))
-    rm, rv, batch_stats, factor = plan
-    fn = _BatchNormAct8 if keeps8 else _BatchNormAct
-    y = fn.apply(z, bn.weight, bn.bias, rm, rv, bn.eps, float(act.negative_slope) if fused_act else None,
-                 batch_stats, factor, col_sums if batch_stats else None)
+    rm, rv, batch_stats, factor, counter = plan
+    slope = float(act.negative_slope) if fused_act else None
+    col_sums = col_sums if batch_stats else None
+    if keeps8:
+        y = _BatchNormAct8.apply(z, bn.weight, bn.bias, rm, rv, bn.eps, slope, batch_stats, factor, counter, col_sums)
+    else:
+        y = _BatchNormAct.apply(z, bn.weight, bn.bias, rm, rv, bn.eps, slope, batch_stats, factor, col_sums)
     return y if fused_act else act(y)
 
 
@@ -359,12 +370,12 @@ def batch_norm_act_linear(z, bn, act, lin, col_sums=None, want_sums=False, keep=
     of the normalised rows between them; elsewhere they are two calls."""
     if (isinstance(act, torch.nn.LeakyReLU) and _takes(lin, z)
             and _keeps8(keep, z, bn.weight, bn.bias, lin.weight, lin.bias)):
-        plan = _bn_plan(z, bn)
+        plan = _bn_plan(z, bn, True)
         if plan is not None:
-            rm, rv, batch_stats, factor = plan
+            rm, rv, batch_stats, factor, counter = plan
             y, sums = _BatchNormActLinear8.apply(
                 z, bn.weight, bn.bias, lin.weight, lin.bias, rm, rv, bn.eps, float(act.negative_slope),
-                batch_stats, factor, col_sums if batch_stats else None, bool(want_sums))
+                batch_stats, factor, counter, col_sums if batch_stats else None, bool(want_sums))
             return (y, sums) if want_sums else y
     return linear(lin, batch_norm_act(z, bn, act, col_sums=col_sums, keep=keep), want_sums, keep=keep)
 
