@@ -48,18 +48,16 @@ struct ResidualArgs {
 // ---- teams ------------------------------------------------------------------------------------
 // A workgroup: teams of TPR lanes, one row each (TPR > 64: one team).
 template <int TPR> struct RnBlock {
-    static constexpr int THREADS = TPR == 128 ? 128 : RN_THREADS;
+    static constexpr int THREADS = RN_THREADS;
     static constexpr int TEAMS = THREADS / TPR;
 };
 // Waves per SIMD a kernel with n channels a lane is compiled for: as many as its registers allow
-// without spills.  A launch fills the chip with exactly that many (a second, partly filled round of
-// workgroups costs as much as a whole one: 262144 x 512 bfloat16 forward 301 us with 768 workgroups
-// of a kernel that fits 768, 387 us with 1024).  Measured, forward: 500000 x 64 float32 at 4, 5, 6, 8
-// waves within 2 %; 262144 x 512 bfloat16 at 3, 4, 5, 6 waves 304, 253, 248, 251 us.  Backward:
-// 500000 x 64 float32 at 3, 4, 5 waves 205, 200, 370 us (spills); 40007 x 1000 bfloat16 at 2, 3 waves
-// 207, 365 us.
-static constexpr int rn_waves_fwd(int n) { return n <= 4 ? 6 : n <= 8 ? 5 : 1; }
-static constexpr int rn_waves_bwd(int n) { return n <= 4 ? 4 : n <= 8 ? 2 : 1; }
+// without spills (the kernels for rows that are not aligned need a few more).  A launch fills the chip
+// with exactly that many: a second, partly filled round of workgroups costs as much as a whole one
+// (262144 x 512 bfloat16 forward 301 us with 768 workgroups of a kernel that fits 768, 387 us with 1024).
+// Backward 500000 x 64 float32 at 3, 4, 5 waves: 205, 200, 370 us (spills).
+static constexpr int rn_waves_fwd(int n) { return n <= 4 ? 6 : n <= 8 ? 4 : n <= 12 ? 3 : 2; }
+static constexpr int rn_waves_bwd(int n) { return n <= 4 ? 4 : n <= 12 ? 2 : 1; }
 
 // lane exchange inside rows of 16 lanes
 template <int CTRL> __device__ __forceinline__ float rn_dpp(float v)
@@ -90,7 +88,7 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float *lds, int &turn)
     for (int i = 0; i < N; ++i) {
         v[i] += rn_dpp<0xb1>(v[i]);         // lane ^ 1
         v[i] += rn_dpp<0x4e>(v[i]);         // lane ^ 2
-        v[i] += rn_dpp<0x141>(v[i]);        // mirrored inside 8
+        if constexpr (TPR >= 8) v[i] += rn_dpp<0x141>(v[i]);        // mirrored inside 8
         if constexpr (TPR >= 16) v[i] += rn_dpp<0x140>(v[i]);       // mirrored inside 16
         if constexpr (TPR >= 32) v[i] = rn_add16(v[i]);
         if constexpr (TPR >= 64) v[i] = rn_add32(v[i]);
@@ -145,13 +143,34 @@ __device__ __forceinline__ void piece_load(const typename R::T *row, int col, in
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = 0u;
-    if (!VEC && col < C) {
-#pragma unroll
-        for (int k = 0; k < W; ++k)
-            if (col + k < C) {
-                if constexpr (W == 4) w[k] = __float_as_uint(row[col + k]);
-                else w[k / 2] |= (unsigned)row[col + k] << (16 * (k & 1));
+    if (!VEC && col < C) {                  // the last C % W channels: 8, 4, 2 bytes (C is the same everywhere)
+        if constexpr (W == 4) {
+            if (C & 2) {
+                const R8Half4 t = *reinterpret_cast<const R8Half4 *>(row + col);
+                w[0] = t.w[0];
+                w[1] = t.w[1];
+                if (C & 1) w[2] = __float_as_uint(row[col + 2]);
+            } else {
+                w[0] = __float_as_uint(row[col]);
             }
+        } else {
+            if (C & 4) {
+                const R8Half4 t = *reinterpret_cast<const R8Half4 *>(row + col);
+                w[0] = t.w[0];
+                w[1] = t.w[1];
+                if (C & 2) {
+                    w[2] = reinterpret_cast<const R8Half2 *>(row + col + 4)->w;
+                    if (C & 1) w[3] = row[col + 6];
+                } else if (C & 1) {
+                    w[2] = row[col + 4];
+                }
+            } else if (C & 2) {
+                w[0] = reinterpret_cast<const R8Half2 *>(row + col)->w;
+                if (C & 1) w[1] = row[col + 2];
+            } else {
+                w[0] = row[col];
+            }
+        }
     }
 }
 
@@ -186,12 +205,31 @@ __device__ __forceinline__ void piece_store(typename R::T *row, int col, int C, 
             *reinterpret_cast<R8Half8 *>(row + col) = t;
         }
     } else if (!VEC && col < C) {
-#pragma unroll
-        for (int k = 0; k < W; ++k)
-            if (col + k < C) {
-                if constexpr (W == 4) row[col + k] = v[k];
-                else row[col + k] = (unsigned short)(w[k / 2] >> (16 * (k & 1)));
+        if constexpr (W == 4) {
+            if (C & 2) {
+                const R8Half4 t = {{w[0], w[1]}};
+                *reinterpret_cast<R8Half4 *>(row + col) = t;
+                if (C & 1) row[col + 2] = v[2];
+            } else {
+                row[col] = v[0];
             }
+        } else {
+            if (C & 4) {
+                const R8Half4 t = {{w[0], w[1]}};
+                *reinterpret_cast<R8Half4 *>(row + col) = t;
+                if (C & 2) {
+                    reinterpret_cast<R8Half2 *>(row + col + 4)->w = w[2];
+                    if (C & 1) row[col + 6] = (unsigned short)w[3];
+                } else if (C & 1) {
+                    row[col + 4] = (unsigned short)w[2];
+                }
+            } else if (C & 2) {
+                reinterpret_cast<R8Half2 *>(row + col)->w = w[0];
+                if (C & 1) row[col + 2] = (unsigned short)w[1];
+            } else {
+                row[col] = (unsigned short)w[0];
+            }
+        }
     }
 }
 
@@ -341,7 +379,7 @@ __device__ __forceinline__ void rn_stats(const float (&v)[NV][W], const RnChanne
     if (t >= 1.17549435e-38f && t < INFINITY) r = __fmaf_rn(0.5f * r, c, r);
 }
 
-template <class R, int NV, bool VEC, int W = RnPiece<R>::W>
+template <class R, int TPR, int NV, bool VEC, int W = RnPiece<R>::W>
 __device__ __forceinline__ void rn_encode(int8_t *codes, uint8_t *exps, i64 row, const int (&col)[NV], int C, const float (&v)[NV][W])
 {
     const int GR = (C + R8_GROUP - 1) / R8_GROUP;
@@ -350,7 +388,7 @@ __device__ __forceinline__ void rn_encode(int8_t *codes, uint8_t *exps, i64 row,
         unsigned m = 0;
 #pragma unroll
         for (int k = 0; k < W; ++k) m = max(m, r8_magnitude(v[j][k]));
-        m = W == 4 ? r8_max8(m) : r8_max4(m);
+        m = W == 4 && TPR >= 8 ? r8_max8(m) : r8_max4(m);         // (a row of 4 lanes is one group)
         const int e = r8_exponent(m, R::E_MAX);
         unsigned q[W / 4];
 #pragma unroll
@@ -430,8 +468,8 @@ __global__ __launch_bounds__(RnBlock<TPR>::THREADS, rn_waves_fwd(NV * RnPiece<R>
             fetch(p, row + stride, adds_next);
             adds_next = seen_at(row + 2 * stride);
         }
-        if (qx) rn_encode<R, NV, VEC>(qx, ex, row, ch.col, C, x);
-        if (qf) rn_encode<R, NV, VEC>(qf, ef, row, ch.col, C, f);
+        if (qx) rn_encode<R, TPR, NV, VEC>(qx, ex, row, ch.col, C, x);
+        if (qf) rn_encode<R, TPR, NV, VEC>(qf, ef, row, ch.col, C, f);
         float r = 1.0f, mu = 0.0f;
         if (adds) {
             if (a.post != RN_NONE) rn_stats<TPR, NV, W>(f, ch, C, a.post, a.eps_post, lds, turn, r, mu);
@@ -780,19 +818,35 @@ __global__ __launch_bounds__(RN_THREADS) void residual_fold_kernel(
     if (d_b_pre) d_b_pre[c] = (float)s[3];
 }
 
-// Team of a row of C channels: the smallest whose lanes hold it in one piece each (float32 in two
-// from 257 channels on), up to a workgroup.  At most 8 channels a lane below 2049, so that a row
-// and the one on its way stay in registers with the channels' weights.
+// Team of a row of C channels, by its pieces of 16 bytes: one to three pieces a lane, so that few lanes
+// are idle (35 pieces on 48 places instead of 64: 300000 x 137 float32 forward 287 -> 204 us) and a row
+// stays inside one wave as long as it can (sums without barriers: 60000 x 600 float32 backward 291 -> 232
+// us).  Backward a lane has one piece where that fills the team: its column sums take four registers a
+// channel (500000 x 64: 166 us with two pieces, 153 with one).
 struct RnShape { int tpr, nv; };
-static RnShape rn_shape(int C, int type)
+static RnShape rn_shape(int C, int type, bool forward)
 {
     const int p = type == R8_F32 ? (C + 3) / 4 : (C + 7) / 8;       // pieces of a row
+    if (p <= 4) return {4, 1};
     if (p <= 8) return {8, 1};
+    if (type == R8_F32) {
+        if (p <= 16) return forward ? RnShape{8, 2} : RnShape{16, 1};
+        if (p <= 24) return {8, 3};
+        if (p <= 32) return forward ? RnShape{16, 2} : RnShape{32, 1};
+        if (p <= 48) return {16, 3};
+        if (p <= 64) return forward ? RnShape{32, 2} : RnShape{64, 1};
+        if (p <= 96) return {32, 3};
+        if (p <= 128) return {64, 2};
+        if (p <= 192) return {64, 3};
+        if (p <= 256) return {64, 4};
+        return p <= 512 ? RnShape{256, 2} : RnShape{256, 4};
+    }
     if (p <= 16) return {16, 1};
     if (p <= 32) return {32, 1};
     if (p <= 64) return {64, 1};
-    if (type != R8_F32) return p <= 128 ? RnShape{128, 1} : p <= 256 ? RnShape{256, 1} : RnShape{256, 2};
-    return p <= 128 ? RnShape{64, 2} : p <= 256 ? RnShape{128, 2} : p <= 512 ? RnShape{256, 2} : RnShape{256, 4};
+    if (p <= 128) return {64, 2};
+    if (p <= 192) return {64, 3};
+    return p <= 256 ? RnShape{256, 1} : RnShape{256, 2};
 }
 
 static unsigned rn_blocks(i64 rows, RnShape shape, int waves, int most)
@@ -801,7 +855,7 @@ static unsigned rn_blocks(i64 rows, RnShape shape, int waves, int most)
     if (hipGetDevice(&dev) != hipSuccess ||
         hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) cus = 256;
     const int teams = shape.tpr > 64 ? 1 : RN_THREADS / shape.tpr;
-    const i64 full = (i64)cus * waves * (shape.tpr == 128 ? 2 : 1);
+    const i64 full = (i64)cus * waves;
     i64 n = (rows + teams - 1) / teams;
     if (n > full) n = full;
     if (n > most) n = most;
@@ -832,11 +886,13 @@ using namespace mvf;
 #define MVF_RN_SHAPES_16(R_, V_)                                                                    \
     do {                                                                                            \
         switch (shape.tpr * 16 + shape.nv) {                                                        \
+        case 4 * 16 + 1: MVF_RN_LAUNCH(R_, 4, 1, V_); break;                                        \
         case 8 * 16 + 1: MVF_RN_LAUNCH(R_, 8, 1, V_); break;                                        \
         case 16 * 16 + 1: MVF_RN_LAUNCH(R_, 16, 1, V_); break;                                      \
         case 32 * 16 + 1: MVF_RN_LAUNCH(R_, 32, 1, V_); break;                                      \
         case 64 * 16 + 1: MVF_RN_LAUNCH(R_, 64, 1, V_); break;                                      \
-        case 128 * 16 + 1: MVF_RN_LAUNCH(R_, 128, 1, V_); break;                                    \
+        case 64 * 16 + 2: MVF_RN_LAUNCH(R_, 64, 2, V_); break;                                      \
+        case 64 * 16 + 3: MVF_RN_LAUNCH(R_, 64, 3, V_); break;                                      \
         case 256 * 16 + 1: MVF_RN_LAUNCH(R_, 256, 1, V_); break;                                    \
         default: MVF_RN_LAUNCH(R_, 256, 2, V_); break;                                              \
         }                                                                                           \
@@ -844,13 +900,16 @@ using namespace mvf;
 #define MVF_RN_SHAPES_32(R_, V_)                                                                    \
     do {                                                                                            \
         switch (shape.tpr * 16 + shape.nv) {                                                        \
+        case 4 * 16 + 1: MVF_RN_LAUNCH(R_, 4, 1, V_); break;                                        \
         case 8 * 16 + 1: MVF_RN_LAUNCH(R_, 8, 1, V_); break;                                        \
-        case 16 * 16 + 1: MVF_RN_LAUNCH(R_, 16, 1, V_); break;                                      \
-        case 32 * 16 + 1: MVF_RN_LAUNCH(R_, 32, 1, V_); break;                                      \
-        case 64 * 16 + 1: MVF_RN_LAUNCH(R_, 64, 1, V_); break;                                      \
+        case 8 * 16 + 3: MVF_RN_LAUNCH(R_, 8, 3, V_); break;                                        \
+        case 16 * 16 + 3: MVF_RN_LAUNCH(R_, 16, 3, V_); break;                                      \
+        case 32 * 16 + 3: MVF_RN_LAUNCH(R_, 32, 3, V_); break;                                      \
         case 64 * 16 + 2: MVF_RN_LAUNCH(R_, 64, 2, V_); break;                                      \
-        case 128 * 16 + 2: MVF_RN_LAUNCH(R_, 128, 2, V_); break;                                    \
+        case 64 * 16 + 3: MVF_RN_LAUNCH(R_, 64, 3, V_); break;                                      \
+        case 64 * 16 + 4: MVF_RN_LAUNCH(R_, 64, 4, V_); break;                                      \
         case 256 * 16 + 2: MVF_RN_LAUNCH(R_, 256, 2, V_); break;                                    \
+        MVF_RN_OWN(R_, V_)                                                                          \
         default: MVF_RN_LAUNCH(R_, 256, 4, V_); break;                                              \
         }                                                                                           \
     } while (0)
@@ -861,6 +920,10 @@ using namespace mvf;
         else { if (vec) MVF_RN_SHAPES_16(RowF16, true); else MVF_RN_SHAPES_16(RowF16, false); }     \
     } while (0)
 
+#define MVF_RN_OWN(R_, V_)                                                                          \
+    case 8 * 16 + 2: MVF_RN_LAUNCH(R_, 8, 2, V_); break;                                            \
+    case 16 * 16 + 2: MVF_RN_LAUNCH(R_, 16, 2, V_); break;                                          \
+    case 32 * 16 + 2: MVF_RN_LAUNCH(R_, 32, 2, V_); break;
 extern "C" int mvf_residual_norm_forward(
     const void *x, const void *f, int32_t type, int64_t rows, int32_t C, const float *gate, int32_t G,
     const uint8_t *seen, const float *scale, int32_t post, const float *w_post, const float *b_post, float eps_post,
@@ -877,7 +940,7 @@ extern "C" int mvf_residual_norm_forward(
                 "residual_norm_forward: codes and exponents belong together");
     const void *const ptrs[] = {x, f, out, h};
     const bool vec = rn_vec(a, type, ptrs, 4) && (uintptr_t)x_codes % 8 == 0 && (uintptr_t)f_codes % 8 == 0;
-    const RnShape shape = rn_shape(C, type);
+    const RnShape shape = rn_shape(C, type, true);
     const dim3 grid(rn_blocks(rows, shape, rn_waves_fwd(shape.nv * (type == R8_F32 ? 4 : 8)), 1 << 30));
     hipStream_t st = (hipStream_t)stream;
 #define MVF_RN_LAUNCH(R_, TPR_, NV_, V_)                                                                          \
@@ -889,6 +952,12 @@ extern "C" int mvf_residual_norm_forward(
     return MVF_OK;
 }
 
+#undef MVF_RN_OWN
+
+#define MVF_RN_OWN(R_, V_)                                                                          \
+    case 16 * 16 + 1: MVF_RN_LAUNCH(R_, 16, 1, V_); break;                                          \
+    case 32 * 16 + 1: MVF_RN_LAUNCH(R_, 32, 1, V_); break;                                          \
+    case 64 * 16 + 1: MVF_RN_LAUNCH(R_, 64, 1, V_); break;
 extern "C" size_t mvf_residual_norm_workspace_bytes(int64_t rows, int32_t C)
 {
     if (rows < 1 || C < 1 || C > RN_MAX_C) return 0;
@@ -922,7 +991,7 @@ extern "C" int mvf_residual_norm_backward(
     MVF_REQUIRE(!columns || rows == 0 || (workspace && workspace_bytes >= mvf_residual_norm_workspace_bytes(rows, C)),
                 "residual_norm_backward: workspace too small");
     hipStream_t st = (hipStream_t)stream;
-    const RnShape shape = rn_shape(C, type);
+    const RnShape shape = rn_shape(C, type, false);
     const dim3 grid(rn_blocks(rows, shape, rn_waves_bwd(shape.nv * (type == R8_F32 ? 4 : 8)), RN_MAX_BLOCKS_BWD));
     float *partial = columns ? (float *)workspace : nullptr;
     if (rows > 0) {
