@@ -11,14 +11,20 @@
 //
 // Bound by HBM (per row of I -> O columns: forward 4 (I + O) + I bytes, backward 4 (I + O) + I, with
 // BatchNorm 4 O + I more).  Structure of mvf_linear.hip: a wave owns tiles of 32 rows, loaded in
-// memory order a tile ahead, parked in its own LDS region and read back as operands.  One workgroup of
-// eight waves per compute unit, two per SIMD: one's vector work fills the other's matrix instructions;
-// for their registers' sake W lies in LDS as well, read four operands at a time.  In memory order a lane has the same four columns in all its
-// pieces (a row of 8, 16, 32 or 64 columns is 2, 4, 8 or 16 pieces of 16 bytes), so BatchNorm's column
-// terms stay in registers, a group of 32 columns is 8 neighbouring lanes, and codes are stored 256
-// bytes at a time.  The weight gradient runs on the bf16 matrix cores with exact parts
+// memory order a tile ahead, parked in its own LDS region and read back as operands.  One workgroup per
+// compute unit, two or three waves per SIMD: one's vector work fills the other's matrix instructions;
+// for their registers' sake W lies in LDS as well, read four operands at a time.  In memory order a
+// lane has the same four columns in all its pieces (a row of 8, 16, 32 or 64 columns is 2, 4, 8 or 16
+// pieces of 16 bytes), so BatchNorm's column terms stay in registers, a group of 32 columns is 8
+// neighbouring lanes, and codes are stored 256 bytes at a time.  The weight gradient runs on the bf16 matrix cores with exact parts
 // (mvf_bf16x3.h): the tile's g column by column out of LDS, cut into three parts; a value read back
 // from 8 bits is one bf16, an activated value three.
+//
+// 2 M rows of 64 -> 64 columns: Linear forward 268 us, backward 232 us (4.3 and 5.0 TB/s); as separate
+// launches (product, packing, grad_x, grad_W) 671 us in all.  Behind BatchNorm forward 340, the sums'
+// pass 323, the grad_z pass 246 us.  The forward without its products takes 220 us, without its
+// packing 268 instead of 288, without storing y 261: memory alone would bound it, and what is left
+// over is matrix and vector work that two waves per SIMD do not hide behind each other.
 #include "mvf_bf16x3.h"
 #include "mvf_bn_kink.h"
 #include "mvf_norm.h"
@@ -26,13 +32,9 @@
 
 namespace mvf {
 
-#ifndef L8F
-#define L8F 512
-#define L8A 512
-#endif
-constexpr int L8_FWD_THREADS = L8F;
-// (two waves per SIMD for 64 -> 64 columns, whose registers allow no third; three elsewhere)
-constexpr int l8_bwd_threads(int KO, int KI, int mode) { return KO <= 4 && KI <= 4 ? 768 : mode == 2 ? L8A : 512; }
+constexpr int L8_FWD_THREADS = 512;         // (a third wave per SIMD gained nothing)
+// (two waves per SIMD where more than 32 columns on a side leave no registers for a third)
+constexpr int l8_bwd_threads(int KO, int KI) { return KO <= 4 && KI <= 4 ? 768 : 512; }
 constexpr int L8_ROWS = 32;                 // rows per tile
 constexpr int L8_MAX_WGS = 256;             // one per compute unit
 
@@ -308,13 +310,13 @@ enum { L8_LINEAR = 0, L8_SUMS = 1, L8_APPLY = 2 };
 
 // O <= 8 KO columns of g (EXACT: 8 KO, a constant), I = 8 KI columns of the kept rows.
 template <int KO, int KI, int MODE, bool EXACT>
-__global__ __launch_bounds__(l8_bwd_threads(KO, KI, MODE)) void linear8_backward_kernel(
+__global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kernel(
     const float *gsrc, int O_, const int8_t *codes, const uint8_t *exps,
     const float *W, i64 rows, L8Bn bn, int want_sums, float *grad,
     float *partial, float *partial_sums, double *partial_bn)
 {
     constexpr int I = 8 * KI, IQ = 2 * KI, GR = I > 32 ? 2 : 1;
-    constexpr int THREADS = l8_bwd_threads(KO, KI, MODE), WAVES = THREADS / 64;
+    constexpr int THREADS = l8_bwd_threads(KO, KI), WAVES = THREADS / 64;
     const int O = EXACT ? 8 * KO : O_;
     constexpr int NI = I > 32 ? 2 : 1, NA = KO > 4 ? 2 : 1;
     constexpr int PITCH_I = I * 4 + 16;
@@ -710,7 +712,7 @@ static int l8_backward(const float *g, int O, const int8_t *codes, const uint8_t
     int nwg = 0;
 #define MVF_L8B(KO_, KI_)                                                                                          \
     do {                                                                                                           \
-        constexpr int threads = l8_bwd_threads(KO_, KI_, MODE);                                                    \
+        constexpr int threads = l8_bwd_threads(KO_, KI_);                                                          \
         nwg = l8_workgroups(rows, threads);                                                                        \
         if (O == 8 * KO_)                                                                                          \
             hipLaunchKernelGGL((linear8_backward_kernel<KO_, KI_, MODE, true>), dim3((unsigned)nwg), dim3(threads), 0, st, \
