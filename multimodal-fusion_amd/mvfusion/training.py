@@ -319,7 +319,7 @@ def _bn_plan(z, bn, kernel_counts=False):
     weight, bias = bn._parameters["weight"], bn._parameters["bias"]
     rm, rv, tracked = (bn._buffers.get(k) for k in ("running_mean", "running_var", "num_batches_tracked"))
     for t in (weight, bias, rm, rv):
-        if t is not None and not (t.is_cuda and t.dtype == torch.float32):
+        if t is not None and not (t.device == z.device and t.dtype == torch.float32):
             return None
     batch_stats = bn.training or rm is None
     factor, counter = 0.0, None
@@ -328,7 +328,7 @@ def _bn_plan(z, bn, kernel_counts=False):
             raise ValueError(
                 f"Expected more than 1 value per channel when training, got input size {tuple(z.shape)}")
         if bn.training and bn.track_running_stats and tracked is not None:
-            if kernel_counts and bn.momentum is not None and tracked.is_cuda and tracked.dtype == torch.int64:
+            if kernel_counts and bn.momentum is not None and tracked.device == z.device and tracked.dtype == torch.int64:
                 counter = tracked
             else:
                 tracked.add_(1)
@@ -531,7 +531,7 @@ class _Linear8(torch.autograd.Function):
 
 def _takes(lin, x):
     return (x.is_cuda and x.dtype == torch.float32 and x.dim() == 2 and x.shape[0] > 0
-            and lin.weight.is_cuda and lin.weight.dtype == torch.float32)
+            and lin.weight.device == x.device and lin.weight.dtype == torch.float32)
 
 
 def _linear(x, weight, bias, want_sums=False, keep=None):

@@ -548,6 +548,44 @@ def test_two_steps_on_two_streams():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("op,I,O", [("linear", 64, 64), ("linear", 65, 8), ("tail", 65, 0), ("block", 64, 64), ("block", 65, 8)])
+def test_more_than_2_31_values(op, I, O):
+    """The last 5000 of 2^25 and some rows as a call on them alone has them.  The other rows' gradients
+    are zeros, which leaves the last rows' in the sums: both calls add the same 5000 terms a column,
+    each off by 5000 u of their magnitudes at most, and the codes of both are the same."""
+    from mvfusion import training as tr
+    rows, last = (1 << 25) + 77, 5000
+    torch.manual_seed(3)
+    lin = torch.nn.Linear(I, O).cuda() if O else None
+    bn = torch.nn.BatchNorm1d(I).cuda().eval()
+    with torch.no_grad():
+        bn.weight.uniform_(0.5, 2)
+        bn.bias.uniform_(-1, 1)
+        bn.running_mean.uniform_(-1, 1)
+        bn.running_var.uniform_(0.5, 2)
+    act = torch.nn.LeakyReLU(0.2)
+    call = {"linear": lambda x: tr.linear(lin, x, keep="int8"),
+            "tail": lambda x: tr.batch_norm_act(x, bn, act, keep="int8"),
+            "block": lambda x: tr.batch_norm_act_linear(x, bn, act, lin, keep="int8")}[op]
+    params = ([] if op == "linear" else [bn.weight, bn.bias]) + ([lin.weight, lin.bias] if O else [])
+    x = torch.randn(rows, I, device="cuda", requires_grad=True)
+    gy = torch.zeros(rows, O or I, device="cuda")
+    gy[-last:].normal_()
+    y = call(x)
+    gx, *sums = torch.autograd.grad(y, [x] + params, gy)
+    xl = x.detach()[-last:].clone().requires_grad_(True)
+    yl = call(xl)
+    gxl, *suml = torch.autograd.grad(yl, [xl] + params, gy[-last:])
+    assert torch.equal(y[-last:], yl)
+    assert torch.equal(gx[-last:], gxl)
+    assert not gx[:1000].any() and not gx[-last - 1000:-last].any()
+    mag = gy[-last:].abs().double().sum(0).max() * xl.detach().abs().double().max().clamp_min(1) * 4
+    if op == "block":       # (BatchNorm's sums: of g W, at most the sum of the weights' magnitudes more)
+        mag = mag * lin.weight.abs().double().sum(0).max().clamp_min(1)
+    for a, b in zip(sums, suml):
+        assert float((a - b).abs().max()) <= 2 * last * U * float(mag)
+
+
 def test_what_autograd_refuses():
     """No second derivative, and no parameter changed between forward and backward."""
     from mvfusion import training as tr
