@@ -41,6 +41,13 @@ template <int PARTS> struct XtyParts {
     }
 };
 
+// The matrix cores add bf16 products to float32 sums by cutting off what does not fit, towards minus
+// infinity: over 2 M rows that shifts sums of zero-mean terms by 2e-6 of their typical size.  Odd
+// waves therefore sum the negated products (one operand's sign turned, by a factor or in its two
+// bf16) and are subtracted where waves are joined: the two halves' errors cancel.
+__device__ __forceinline__ float xty_turned(int wave) { return wave & 1 ? -1.0f : 1.0f; }
+__device__ __forceinline__ unsigned xty_flip(int wave) { return wave & 1 ? 0x80008000u : 0u; }
+
 // Adds up the partial results of nwg workgroups: partial [nwg][NA * NB * 1024] accumulators of NA x NB
 // blocks of 32 x 32 sums as v_mfma_f32_32x32x16_bf16 leaves them (vx / vy: an operand of two blocks holds
 // columns 2 n and 2 n + 1 in lane n), out [A][ldo], and with partial_sums [nwg][64] the sums [A].

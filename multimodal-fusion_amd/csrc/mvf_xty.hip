@@ -297,6 +297,9 @@ __global__ __launch_bounds__(XTY_THREADS) void xty8_kernel(
         const int c = VQ ? 2 * n + i : 32 * i + n;
         qc[i] = c < B ? c : 0;
     }
+    // odd waves sum -x^T y (mvf_bf16x3.h)
+    const float turned = xty_turned(wave);
+    const unsigned flip = xty_flip(wave);
     float gamma[NB], beta[NB];
     BnKink kink[NB];
     if constexpr (TAIL) {
@@ -380,11 +383,14 @@ __global__ __launch_bounds__(XTY_THREADS) void xty8_kernel(
                 v[k] = r8_decode(s.q[j][k], s.e[VQ ? 0 : j][k]);
                 if constexpr (TAIL) {
                     const float a = __fmaf_rn(v[k], gamma[j], beta[j]);
-                    v[k] = (tail.act && !kink[j].on(v[k])) ? a * tail.slope : a;
+                    v[k] = a * ((tail.act && !kink[j].on(v[k])) ? turned * tail.slope : turned);
                 }
             }
             XtyParts<TAIL ? 3 : 1> yp;
             yp.cut(v);
+            if constexpr (!TAIL)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) yp.p[0][h] ^= flip;
 #pragma unroll
             for (int i = 0; i < NA; ++i) {
                 if constexpr (TAIL) {
@@ -446,7 +452,7 @@ __global__ __launch_bounds__(XTY_THREADS) void xty8_kernel(
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const int at = ((i * NB + j) * 16 + e) * 64 + lane;
-                        fold[at] = turn == 0 ? acc[i][j][e] : fold[at] + acc[i][j][e];
+                        fold[at] = turn == 0 ? acc[i][j][e] : __fmaf_rn(turned, acc[i][j][e], fold[at]);
                     }
         }
         __syncthreads();

@@ -548,6 +548,32 @@ def test_two_steps_on_two_streams():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("O", [64, 60])
+@pytest.mark.parametrize("tail", [False, True])
+def test_weight_gradient_has_no_common_shift(tail, O):
+    """Sums of many zero-mean terms: the matrix cores' rounding, which goes one way, must not move all of
+    them together.  The errors of the 64 O sums share 64 and O columns, so the mean of unbiased
+    ones is within about std / 7.7 of zero; half the deviation is nearly four times that."""
+    from mvfusion import training as tr
+    rows = 1 << 20
+    torch.manual_seed(5)
+    lin, bn, act = torch.nn.Linear(64, O).cuda(), torch.nn.BatchNorm1d(64).cuda(), torch.nn.LeakyReLU(0.2)
+    x, gy = torch.randn(rows, 64, device="cuda", requires_grad=True), torch.randn(rows, O, device="cuda")
+    y = tr.batch_norm_act_linear(x, bn, act, lin, keep="int8") if tail else tr.linear(lin, x, keep="int8")
+    _, gw = torch.autograd.grad(y, (x, lin.weight), gy)
+    from mvfusion import packed
+    if tail:
+        _, codes, exps, _ = tr._bn8_forward(x.detach(), bn.weight.detach(), bn.bias.detach(), None, None, bn.eps, 0.2,
+                                            True, 0.0, None, None)
+        v = packed.unpack_rows(codes, exps).double()
+        v = torch.where(v > 0, v, v * float(np.float32(0.2)))
+    else:
+        v = packed.pack_rows(x).unpack().double()
+    g = gy.double().view(-1, 512, O).transpose(1, 2).contiguous()
+    err = gw.double() - torch.bmm(g, v.view(-1, 512, 64)).sum(0)
+    assert abs(float(err.mean())) <= 0.5 * float(err.std())
+
+
 @pytest.mark.parametrize("op,I,O", [("linear", 64, 64), ("linear", 65, 8), ("tail", 65, 0), ("block", 64, 64), ("block", 65, 8)])
 def test_more_than_2_31_values(op, I, O):
     """The last 5000 of 2^25 and some rows as a call on them alone has them.  The other rows' gradients
@@ -581,7 +607,7 @@ def test_more_than_2_31_values(op, I, O):
     assert not gx[:1000].any() and not gx[-last - 1000:-last].any()
     mag = gy[-last:].abs().double().sum(0).max() * xl.detach().abs().double().max().clamp_min(1) * 4
     if op == "block":       # (BatchNorm's sums: of g W, at most the sum of the weights' magnitudes more)
-        mag = mag * lin.weight.abs().double().sum(0).max().clamp_min(1)
+        mag = mag * lin.weight.detach().abs().double().sum(0).max().clamp_min(1)
     for a, b in zip(sums, suml):
         assert float((a - b).abs().max()) <= 2 * last * U * float(mag)
 
