@@ -20,11 +20,13 @@
 // (mvf_bf16x3.h): the tile's g column by column out of LDS, cut into three parts; a value read back
 // from 8 bits is one bf16, an activated value three.
 //
-// 2 M rows of 64 -> 64 columns: Linear forward 268 us, backward 232 us (4.3 and 5.0 TB/s); as separate
-// launches (product, packing, grad_x, grad_W) 671 us in all.  Behind BatchNorm forward 340, the sums'
-// pass 323, the grad_z pass 246 us.  The forward without its products takes 220 us, without its
-// packing 268 instead of 288, without storing y 261: memory alone would bound it, and what is left
-// over is matrix and vector work that two waves per SIMD do not hide behind each other.
+// 2 M rows of 64 -> 64 columns: a Linear forward and backward 500 us (4.6 TB/s; as separate launches of
+// product, packing, grad_x and grad_W 671 us); behind BatchNorm 920 us, of which the kernel trace gives
+// the statistics 90, the forward 342, the sums' pass 336 and the grad_z pass 237 us.  Not bound by
+// memory alone: the Linear's forward takes 288 us in the trace, 268 without its packing, 261
+// without storing y and 220 without its products.  In the sums' pass the matrix units are busy for 143
+// us and the vector units for 118; two waves per SIMD leave the two, and the way through LDS, one
+// behind the other, and the registers allow no third (wave priorities around the products: nothing).
 #include "mvf_bf16x3.h"
 #include "mvf_bn_kink.h"
 #include "mvf_norm.h"
@@ -599,11 +601,14 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
         }
         l8_wave_sync();
     };
+    // grad_z's pass goes from the last tile to the first: the memory-side cache still holds the end of what the
+    // sums' pass has read (2 M rows of 64 columns: 240 -> 235 us)
+    auto at = [&](i64 t) { return MODE == L8_APPLY ? nfull - 1 - t : t; };
     if (wid < nfull) {
-        load_tile(wid, L8_ROWS);
+        load_tile(at(wid), L8_ROWS);
         i64 t = wid;
-        tile(t, L8_ROWS, t + nwaves < nfull ? t + nwaves : t, L8Tile<true, true>());
-        for (t += nwaves; t < nfull; t += nwaves) tile(t, L8_ROWS, t + nwaves < nfull ? t + nwaves : t, L8Tile<true, true>());
+        tile(at(t), L8_ROWS, at(t + nwaves < nfull ? t + nwaves : t), L8Tile<true, true>());
+        for (t += nwaves; t < nfull; t += nwaves) tile(at(t), L8_ROWS, at(t + nwaves < nfull ? t + nwaves : t), L8Tile<true, true>());
     }
     if (rest > 0 && wid == nfull % nwaves) {
         load_tile(nfull, rest);
