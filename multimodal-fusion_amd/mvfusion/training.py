@@ -377,7 +377,8 @@ def batch_norm_act_linear(z, bn, act, lin, col_sums=None, want_sums=False, keep=
                 z, bn.weight, bn.bias, lin.weight, lin.bias, rm, rv, bn.eps, float(act.negative_slope),
                 batch_stats, factor, counter, col_sums if batch_stats else None, bool(want_sums))
             return (y, sums) if want_sums else y
-    return linear(lin, batch_norm_act(z, bn, act, col_sums=col_sums, keep=keep), want_sums, keep=keep)
+    form = {} if keep is None else {"keep": keep}
+    return linear(lin, batch_norm_act(z, bn, act, col_sums=col_sums, **form), want_sums, **form)
 
 
 def xty(x, y=None):

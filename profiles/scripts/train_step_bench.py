@@ -1,6 +1,7 @@
 """One training step (forward + backward) of QKVBimodalCSRPool at C3 size, with the
 BatchNorm1d + LeakyReLU tails and the weight gradients of the dense layers on this
-library's kernels (training.batch_norm_act, training.linear) and on the torch modules."""
+library's kernels (training.batch_norm_act, training.linear), with those keeping 8-bit rows
+for the backward (training.keep_activations), and on the torch modules."""
 import os
 import sys
 import numpy as np
@@ -35,17 +36,19 @@ def step():
     out.sum().backward()
 
 
-for name, fns in (("kernels", own), ("torch modules", plain), ("kernels", own)):
+for name, fns, form in (("kernels", own, "float32"), ("torch modules", plain, "float32"),
+                        ("kernels, 8-bit rows kept", own, "int8"), ("kernels", own, "float32")):
     training.batch_norm_act, training.linear = fns
-    for _ in range(3):
-        step()
-    torch.cuda.synchronize()
-    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-    e0.record()
-    for _ in range(10):
-        step()
-    e1.record()
-    torch.cuda.synchronize()
+    with training.keep_activations(form):
+        for _ in range(3):
+            step()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        for _ in range(10):
+            step()
+        e1.record()
+        torch.cuda.synchronize()
     print(f"{name}: {e0.elapsed_time(e1) / 10:.2f} ms per training step ({Vw} rows), "
           f"peak memory {torch.cuda.max_memory_allocated() / 2**20:.0f} MiB")
-    torch.cuda.reset_peak_memory_stats()
