@@ -5,9 +5,8 @@
 //             normalised z): the activated rows exist in LDS only.  The products and their order
 //             are those of mvf_linear.hip: the same bits.
 //   backward  of the Linear: grad_x = g W, grad_W = g^T xq and grad_b = sum g from one read of g;
-//             of BatchNorm + LeakyReLU + Linear: a pass that leaves grad_W (of the activated rows made
-//             of the codes again) and the column sums of BatchNorm's backward, and a pass that writes
-//             grad_z; both form g W, which is never stored.
+//             of BatchNorm + LeakyReLU + Linear: a pass of reductions that leaves grad_W and the column sums
+//             of BatchNorm's backward, and a pass that forms g W and writes grad_z.
 //
 // Bound by HBM (per row of I -> O columns: forward 4 (I + O) + I bytes, backward 4 (I + O) + I, with
 // BatchNorm 4 O + I more).  Structure of mvf_linear.hip: a wave owns tiles of 32 rows, loaded in
@@ -16,17 +15,17 @@
 // for their registers' sake W lies in LDS as well, read four operands at a time.  In memory order a
 // lane has the same four columns in all its pieces (a row of 8, 16, 32 or 64 columns is 2, 4, 8 or 16
 // pieces of 16 bytes), so BatchNorm's column terms stay in registers, a group of 32 columns is 8
-// neighbouring lanes, and codes are stored 256 bytes at a time.  The weight gradient runs on the bf16 matrix cores with exact parts
-// (mvf_bf16x3.h): the tile's g column by column out of LDS, cut into three parts; a value read back
-// from 8 bits is one bf16, an activated value three.
+// neighbouring lanes, and codes are stored 256 bytes at a time.  The weight gradient runs on the bf16
+// matrix cores with exact parts (mvf_bf16x3.h): the tile's g column by column out of LDS, cut into three
+// parts; a value read back from 8 bits is one bf16.
 //
 // 2 M rows of 64 -> 64 columns: a Linear forward and backward 500 us (4.6 TB/s; as separate launches of
-// product, packing, grad_x and grad_W 671 us); behind BatchNorm 920 us, of which the kernel trace gives
-// the statistics 90, the forward 342, the sums' pass 336 and the grad_z pass 237 us.  Not bound by
+// product, packing, grad_x and grad_W 671 us); behind BatchNorm 800 us, of which the kernel trace gives
+// the statistics 90, the forward 342, the sums' pass 203 and the grad_z pass 237 us.  Not bound by
 // memory alone: the Linear's forward takes 288 us in the trace, 268 without its packing, 261
-// without storing y and 220 without its products.  In the sums' pass the matrix units are busy for 143
-// us and the vector units for 118; two waves per SIMD leave the two, and the way through LDS, one
-// behind the other, and the registers allow no third (wave priorities around the products: nothing).
+// without storing y and 220 without its products.  Two waves per SIMD leave matrix and vector work, and
+// the way through LDS, partly one behind the other, and the registers allow no third (wave
+// priorities around the products: nothing).
 #include "mvf_bf16x3.h"
 #include "mvf_bn_kink.h"
 #include "mvf_norm.h"
@@ -37,6 +36,7 @@ namespace mvf {
 constexpr int L8_FWD_THREADS = 512;         // (a third wave per SIMD gained nothing)
 // (two waves per SIMD where more than 32 columns on a side leave no registers for a third)
 constexpr int l8_bwd_threads(int KO, int KI) { return KO <= 4 && KI <= 4 ? 768 : 512; }
+constexpr int T8_THREADS = 512;
 constexpr int L8_ROWS = 32;                 // rows per tile
 constexpr int L8_MAX_WGS = 256;             // one per compute unit
 
@@ -308,14 +308,14 @@ __global__ __launch_bounds__(L8_FWD_THREADS) void linear8_forward_kernel(
 }
 
 // ---- backward ---------------------------------------------------------------------------------
-enum { L8_LINEAR = 0, L8_SUMS = 1, L8_APPLY = 2 };
+enum { L8_LINEAR = 0, L8_APPLY = 1 };
 
 // O <= 8 KO columns of g (EXACT: 8 KO, a constant), I = 8 KI columns of the kept rows.
 template <int KO, int KI, int MODE, bool EXACT>
 __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kernel(
     const float *gsrc, int O_, const int8_t *codes, const uint8_t *exps,
     const float *W, i64 rows, L8Bn bn, int want_sums, float *grad,
-    float *partial, float *partial_sums, double *partial_bn)
+    float *partial, float *partial_sums)
 {
     constexpr int I = 8 * KI, IQ = 2 * KI, GR = I > 32 ? 2 : 1;
     constexpr int THREADS = l8_bwd_threads(KO, KI), WAVES = THREADS / 64;
@@ -328,8 +328,7 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
     constexpr int TILE = L8_ROWS * ((KO * 8 > I ? KO * 8 : I) * 4 + 16);
     constexpr int REGION = TILE + (XTY ? PLANE : 0);
     constexpr int FOLD = XTY ? (NA * NI * 1024 + WAVES * 64) * 4 : 0;
-    constexpr int RED = MODE == L8_SUMS ? WAVES * 2 * I * 8 : 0;
-    constexpr int LDS = WAVES * REGION > FOLD + RED ? WAVES * REGION : FOLD + RED;
+    constexpr int LDS = WAVES * REGION > FOLD ? WAVES * REGION : FOLD;
     __shared__ __attribute__((aligned(16))) char lds[LDS];
     __shared__ __attribute__((aligned(16))) char wlds[32 * NI * PITCH_W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -356,33 +355,23 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
     const int col = 4 * (lane % IQ), row0 = lane / IQ;
     float scale[4], m_g[4], m_gz[4];
     BnKink kink[4];
-    if constexpr (MODE != L8_LINEAR) {
+    if constexpr (MODE == L8_APPLY) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float gamma = bn.weight ? bn.weight[col + k] : 1.0f;
             kink[k].load(gamma, bn.bias ? bn.bias[col + k] : 0.0f);
             if (!bn.act) kink[k].sign = 0.0f, kink[k].at = -1.0f;       // (every number is on)
-            if constexpr (MODE == L8_APPLY) {
-                scale[k] = gamma * bn.invstd[col + k];
-                m_g[k] = bn.training ? bn.col_terms[col + k] : 0.0f;
-                m_gz[k] = bn.training ? bn.col_terms[I + col + k] : 0.0f;
-            }
+            scale[k] = gamma * bn.invstd[col + k];
+            m_g[k] = bn.training ? bn.col_terms[col + k] : 0.0f;
+            m_gz[k] = bn.training ? bn.col_terms[I + col + k] : 0.0f;
         }
     }
     // columns of g for the weight gradient (past O: column 0, never stored)
     const int gc = NA == 2 ? (2 * n < O ? 2 * n : 0) : (n < O ? n : 0);
     const int qc = NI == 2 ? 2 * n : (n < I ? n : 0);
-    float xgamma[NI], xbeta[NI];            // BatchNorm's terms of the lane's columns there
-    if constexpr (MODE == L8_SUMS) {
-#pragma unroll
-        for (int b = 0; b < NI; ++b) {
-            xgamma[b] = bn.weight ? bn.weight[qc + b] : 1.0f;
-            xbeta[b] = bn.bias ? bn.bias[qc + b] : 0.0f;
-        }
-    }
     // odd waves sum -g^T y (mvf_bf16x3.h)
-    const float turned = xty_turned(wave);
-    const unsigned flip = xty_flip(wave);
+    [[maybe_unused]] const float turned = xty_turned(wave);
+    [[maybe_unused]] const unsigned flip = xty_flip(wave);
     xty_acc run[XTY ? NA : 1][XTY ? NI : 1];
     float sums[NA];
     if constexpr (XTY) {
@@ -395,12 +384,6 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
                 for (int e = 0; e < 16; ++e) run[i][b][e] = 0.0f;
         }
     }
-    double bs[MODE == L8_SUMS ? 4 : 1], bq[MODE == L8_SUMS ? 4 : 1];
-    if constexpr (MODE == L8_SUMS) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) bs[k] = bq[k] = 0.0;
-    }
-
     const i64 nfull = rows / L8_ROWS;
     const int rest = (int)(rows - nfull * L8_ROWS);
     const i64 wid = (i64)blockIdx.x * WAVES + wave, nwaves = (i64)gridDim.x * WAVES;
@@ -448,14 +431,12 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
             }
         }
         l8_wave_sync();
-        // g^T y: lane = column, 8 rows of 16.  With three parts of y a tile's products start from zero and
-        // are added to the running sums afterwards (one rounding of the sums a tile instead of twelve: grad_W
-        // over 2 M rows off by 1.5e-7 instead of 4.7e-7, in the same time).
+        // g^T y: lane = column, 8 rows of 16
         if constexpr (XTY) {
-            XtyParts<3> gp[2][NA];
-            unsigned d[2][8];
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
+                XtyParts<3> gp[NA];
+                unsigned d[8];
                 float c[NA][8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
@@ -468,58 +449,24 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
                         c[0][k] = *(const float *)at;
                     }
                     const char *qt = plane + (16 * st + 8 * kh + k) * PITCH_Q + qc * 2;
-                    d[st][k] = NI == 2 ? *(const unsigned *)qt : (unsigned)*(const unsigned short *)qt;
+                    d[k] = NI == 2 ? *(const unsigned *)qt : (unsigned)*(const unsigned short *)qt;
                 }
 #pragma unroll
                 for (int i = 0; i < NA; ++i) {
-                    gp[st][i].cut(c[i]);
+                    gp[i].cut(c[i]);
                     if (want_sums)
                         sums[i] += ((c[i][0] + c[i][1]) + (c[i][2] + c[i][3])) + ((c[i][4] + c[i][5]) + (c[i][6] + c[i][7]));
                 }
-                if constexpr (MODE == L8_LINEAR) {
-#pragma unroll
-                    for (int b = 0; b < NI; ++b) {
-                        xty_u4 yp;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            yp[k] = __builtin_amdgcn_perm(d[st][2 * k + 1], d[st][2 * k], b == 0 ? 0x05040100u : 0x07060302u) ^ flip;
-#pragma unroll
-                        for (int p = 2; p >= 0; --p)
-#pragma unroll
-                            for (int i = 0; i < NA; ++i) run[i][b] = xty_mfma16(gp[st][i].p[p], yp, run[i][b]);
-                    }
-                }
-            }
-            if constexpr (MODE == L8_SUMS) {
 #pragma unroll
                 for (int b = 0; b < NI; ++b) {
-                    xty_acc tmp[NA];
+                    xty_u4 yp;
 #pragma unroll
-                    for (int i = 0; i < NA; ++i)
+                    for (int k = 0; k < 4; ++k)
+                        yp[k] = __builtin_amdgcn_perm(d[2 * k + 1], d[2 * k], b == 0 ? 0x05040100u : 0x07060302u) ^ flip;
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) tmp[i][k] = 0.0f;
+                    for (int p = 2; p >= 0; --p)
 #pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        float v[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float zq = __uint_as_float(b == 0 ? d[st][k] << 16 : d[st][k] & 0xffff0000u);
-                            const float a = __fmaf_rn(zq, xgamma[b], xbeta[b]);
-                            v[k] = a * (a > 0.0f ? turned : turned * bn.slope);
-                        }
-                        XtyParts<3> yp;
-                        yp.cut(v);
-                        // (the parts' products in ascending size)
-                        constexpr int pg[6] = {2, 1, 0, 1, 0, 0}, py[6] = {0, 1, 2, 0, 1, 0};
-#pragma unroll
-                        for (int p = 0; p < 6; ++p)
-#pragma unroll
-                            for (int i = 0; i < NA; ++i) tmp[i] = xty_mfma16(gp[st][i].p[pg[p]], yp.p[py[p]], tmp[i]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < NA; ++i)
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) run[i][b][k] += tmp[i][k];
+                        for (int i = 0; i < NA; ++i) run[i][b] = xty_mfma16(gp[i].p[p], yp, run[i][b]);
                 }
             }
         }
@@ -565,39 +512,20 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
                 }
             }
         l8_wave_sync();
-        l8_f4 *dst = (l8_f4 *)(grad + (MODE != L8_SUMS ? (size_t)t * L8_ROWS * I : 0));
-        float ts[4] = {0.0f, 0.0f, 0.0f, 0.0f}, tq[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        l8_f4 *dst = (l8_f4 *)(grad + (size_t)t * L8_ROWS * I);
 #pragma unroll
         for (int j = 0; j < KI; ++j) {
             const int r = row0 + j * (64 / IQ);
             l8_f4 v = *(const l8_f4 *)(buf + r * PITCH_I + col * 4);
-            if constexpr (MODE != L8_LINEAR) {
-                r8_u2 d;
-                if constexpr (XTY) d = *(const r8_u2 *)(plane + r * PITCH_Q + col * 2);
+            if constexpr (MODE == L8_APPLY) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    float zq;
-                    if constexpr (XTY) zq = __uint_as_float(k & 1 ? d[k / 2] & 0xffff0000u : d[k / 2] << 16);
-                    else zq = r8_decode(r8_byte(q[j], k), e[j]);
+                    const float zq = r8_decode(r8_byte(q[j], k), e[j]);
                     const float gg = kink[k].on(zq) ? v[k] : v[k] * bn.slope;
-                    if constexpr (MODE == L8_SUMS) {
-                        ts[k] += gg;
-                        tq[k] = __fmaf_rn(gg, zq, tq[k]);
-                    } else {
-                        v[k] = bn.training ? (gg - m_g[k] - zq * m_gz[k]) * scale[k] : gg * scale[k];
-                    }
+                    v[k] = bn.training ? (gg - m_g[k] - zq * m_gz[k]) * scale[k] : gg * scale[k];
                 }
             }
-            if constexpr (MODE != L8_SUMS) {
-                if (WHOLE || r < live) r8_stream(dst + lane + 64 * j, v);
-            }
-        }
-        if constexpr (MODE == L8_SUMS) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                bs[k] += (double)ts[k];
-                bq[k] += (double)tq[k];
-            }
+            if (WHOLE || r < live) r8_stream(dst + lane + 64 * j, v);
         }
         l8_wave_sync();
     };
@@ -649,28 +577,253 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
             }
         }
     }
-    if constexpr (MODE == L8_SUMS) {
-        double *red = (double *)(lds + FOLD);
+}
+
+// The sums' pass behind BatchNorm + LeakyReLU, a reduction over the rows alone.  With on = 1 above the kink
+// and 0 below, zq the rows read back and s the slope, what the activation passes on of a gradient is
+// t = s + (1 - s) on of it, and the Linear's input is t (gamma zq + beta).  So with
+//   P = g^T (t zq) = s g^T zq + (1 - s) g^T (on zq),      Q = g^T t = s sum g + (1 - s) g^T on
+// grad_W = gamma P + beta Q, and BatchNorm's column sums, of t (g W) and t (g W) zq, are the columns of
+// W . Q and W . P: neither g W nor the activated rows are formed.  zq, on zq and on are exact in one bf16, so
+// the three products are nine of the bf16 matrix cores', exact but for their float32 sums.  2 M rows of
+// 64 -> 64 columns take 203 us (with g W and the activated rows formed: 337), 161 of them without the
+// products, 128 for the bytes.  Past 32 columns of g two waves share a tile, 32 columns each: three sums of
+// 64 x 64 would leave room for one wave per SIMD (four waves a tile, of 32 x 32 sums: 227 to 253 us).
+template <int KO, int KI, bool EXACT>
+__global__ __launch_bounds__(T8_THREADS) void tail8_sums_kernel(
+    const float *gsrc, int O_, const int8_t *codes, const uint8_t *exps, i64 rows, L8Bn bn, float *partial, float *partial_sums)
+{
+    constexpr int I = 8 * KI, IQ = 2 * KI, GR = I > 32 ? 2 : 1;
+    constexpr int WAVES = T8_THREADS / 64;
+    constexpr int NA = KO > 4 ? 2 : 1, NI = I > 32 ? 2 : 1, UNITS = WAVES / NA;
+    constexpr int GP = NA == 2 ? 4 : KO;                    // pieces of g a lane loads
+    constexpr int PITCH_G = 32 * GP + 16, TILE = L8_ROWS * PITCH_G;
+    constexpr int PITCH_Q = I * 2 + 16, REGION = TILE + L8_ROWS * PITCH_Q;
+    constexpr int SLOTS = NA * NI * 1024;                   // sums of one product
+    constexpr int FOLD = (3 * SLOTS + WAVES * 32) * 4;
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * REGION > FOLD ? WAVES * REGION : FOLD];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, kh = lane >> 5;
+    const int unit = wave / NA, h = wave % NA;              // (the waves of a tile, the wave's half of g)
+    const int O = EXACT ? 8 * KO : O_;
+    const int width = NA == 1 ? O : h == 0 || EXACT ? 32 : O - 32, gq = width >> 2;
+    char *buf = lds + wave * REGION, *plane = buf + TILE;
+    const int gc = n < width ? n : 0;                       // (past the width: column 0, left out of the fold)
+    const int qc = NI == 2 ? 2 * n : (n < I ? n : 0);
+    // the columns' kinks for rows with the sign of gamma taken in: on where sign zq > at
+    unsigned signs = 0u;
+    float at[NI];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+    for (int b = 0; b < NI; ++b) {
+        const float gamma = bn.weight ? bn.weight[qc + b] : 1.0f, beta = bn.bias ? bn.bias[qc + b] : 0.0f;
+        BnKink kink;
+        kink.load(gamma, beta);
+        if (gamma < 0.0f) signs |= b == 0 ? 0x8000u : 0x80000000u;
+        at[b] = !bn.act ? -__builtin_inff() : gamma != 0.0f ? kink.at : beta > 0.0f ? -__builtin_inff() : __builtin_inff();
+    }
+    // where the lane's pieces of g come from and go to
+    unsigned from[GP], to[GP];
 #pragma unroll
-            for (int d = IQ; d < 64; d <<= 1) {
-                bs[k] += __shfl_xor(bs[k], d, 64);
-                bq[k] += __shfl_xor(bq[k], d, 64);
+    for (int j = 0; j < GP; ++j) {
+        const unsigned f = min((unsigned)lane + 64u * j, (unsigned)(L8_ROWS * gq - 1)), r = f / (unsigned)gq;
+        from[j] = (r * (unsigned)O + 32u * h + (f - r * gq) * 4u) * 4u;
+        to[j] = r * PITCH_G + (f - r * gq) * 16u;
+    }
+    const int col = 4 * (lane % IQ), row0 = lane / IQ;      // the lane's codes in memory order
+    xty_acc all[NI], above[NI], on[NI];                     // of sign zq, on sign zq, on
+    float sums = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NI; ++b)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) all[b][k] = above[b][k] = on[b][k] = 0.0f;
+
+    const i64 nfull = rows / L8_ROWS;
+    const int rest = (int)(rows - nfull * L8_ROWS);
+    const i64 uid = (i64)blockIdx.x * UNITS + unit, nunits = (i64)gridDim.x * UNITS;
+    const float turned = xty_turned((int)uid);              // odd units sum -g^T (...) (mvf_bf16x3.h)
+    l8_f4 g[GP];
+    unsigned qw[KI];
+    int ew;
+    auto load_tile = [&](i64 t, int live) {
+        const char *src = (const char *)(gsrc + (size_t)t * L8_ROWS * O);
+        const unsigned last = ((unsigned)(live - 1) * O + 32u * h) * 4u;
+#pragma unroll
+        for (int j = 0; j < GP; ++j)
+            g[j] = *(const l8_f4 *)(src + (live == L8_ROWS || lane + 64 * j < live * gq ? from[j] : last));
+        const unsigned *qsrc = (const unsigned *)(codes + (size_t)t * L8_ROWS * I);
+#pragma unroll
+        for (int j = 0; j < KI; ++j) {
+            const int f = lane + 64 * j;
+            qw[j] = qsrc[live == L8_ROWS || f < live * IQ ? f : live * IQ - 1];
+        }
+        ew = exps[(size_t)t * L8_ROWS * GR + (lane < live * GR ? lane : live * GR - 1)];
+    };
+    auto tile = [&](int live, i64 next, auto how) {
+        constexpr bool WHOLE = decltype(how)::WHOLE;
+#pragma unroll
+        for (int j = 0; j < GP; ++j) {
+            const int f = lane + 64 * j;
+            const l8_f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (EXACT || f < L8_ROWS * gq) *(l8_f4 *)(buf + to[j]) = WHOLE || f < live * gq ? g[j] * turned : zero;
+        }
+        // the kept rows as they read back, one bf16 each; codes of NaN are looked for in all of them at once
+        int e[KI];
+        float least = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KI; ++j) {
+            e[j] = __shfl(ew, (row0 + j * (64 / IQ)) * GR + col / R8_GROUP, 64);
+            const float step = ldexpf(1.0f, e[j] - R8_BIAS);
+            float c[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) c[k] = (float)r8_byte(qw[j], k);
+            least = fminf(fminf(least, c[0]), c[1]);
+            least = fminf(fminf(least, c[2]), c[3]);
+            const r8_u2 d = {xty_hi2(c[0] * step, c[1] * step), xty_hi2(c[2] * step, c[3] * step)};
+            *(r8_u2 *)(plane + (row0 + j * (64 / IQ)) * PITCH_Q + col * 2) = d;
+        }
+        if (__any(least == (float)R8_NAN)) {
+#pragma unroll
+            for (int j = 0; j < KI; ++j) {
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = r8_decode(r8_byte(qw[j], k), e[j]);
+                const r8_u2 d = {xty_hi2(v[0], v[1]), xty_hi2(v[2], v[3])};
+                *(r8_u2 *)(plane + (row0 + j * (64 / IQ)) * PITCH_Q + col * 2) = d;
             }
-        if (lane < IQ)
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (decltype(how)::NEXT) load_tile(next, L8_ROWS);
+        __builtin_amdgcn_sched_barrier(0);
+        l8_wave_sync();
+        // lane = column, 8 rows of 16
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                red[(wave * 2) * I + col + k] = bs[k];
-                red[(wave * 2 + 1) * I + col + k] = bq[k];
+        for (int st = 0; st < 2; ++st) {
+            float c[8];
+            unsigned d[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int r = 16 * st + 8 * kh + k;
+                c[k] = *(const float *)(buf + r * PITCH_G + gc * 4);
+                const char *qt = plane + r * PITCH_Q + qc * 2;
+                d[k] = (NI == 2 ? *(const unsigned *)qt : (unsigned)*(const unsigned short *)qt) ^ signs;
             }
+            sums += ((c[0] + c[1]) + (c[2] + c[3])) + ((c[4] + c[5]) + (c[6] + c[7]));
+            XtyParts<3> gp;
+            gp.cut(c);
+#pragma unroll
+            for (int b = 0; b < NI; ++b) {
+                xty_u4 zp, ap, op;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const unsigned lo = d[2 * k], hi = d[2 * k + 1];
+                    zp[k] = __builtin_amdgcn_perm(hi, lo, b == 0 ? 0x05040100u : 0x07060302u);
+                    unsigned up = __uint_as_float(b == 0 ? lo << 16 : lo & 0xffff0000u) > at[b] ? 0xffffu : 0u;
+                    up = __uint_as_float(b == 0 ? hi << 16 : hi & 0xffff0000u) > at[b] ? up | 0xffff0000u : up;
+                    ap[k] = zp[k] & up;
+                    op[k] = 0x3f803f80u & up;               // (1.0 twice)
+                }
+#pragma unroll
+                for (int p = 2; p >= 0; --p) {
+                    all[b] = xty_mfma16(gp.p[p], zp, all[b]);
+                    above[b] = xty_mfma16(gp.p[p], ap, above[b]);
+                    on[b] = xty_mfma16(gp.p[p], op, on[b]);
+                }
+            }
+        }
+        l8_wave_sync();
+    };
+    if (uid < nfull) {
+        load_tile(uid, L8_ROWS);
+        for (i64 t = uid; t < nfull; t += nunits) tile(L8_ROWS, t + nunits < nfull ? t + nunits : t, L8Tile<true, true>());
+    }
+    if (rest > 0 && uid == nfull % nunits) {
+        load_tile(nfull, rest);
+        tile(rest, 0, L8Tile<false, false>());
+    }
+
+    // the units joined in their order
+    __syncthreads();
+    float *fold = (float *)lds, *fold_sums = fold + 3 * SLOTS;
+    for (int turn = 0; turn < UNITS; ++turn) {
+        if (unit == turn) {
+#pragma unroll
+            for (int b = 0; b < NI; ++b)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int slot = ((h * NI + b) * 16 + k) * 64 + lane;
+                    fold[slot] = __fmaf_rn(turned, all[b][k], turn == 0 ? 0.0f : fold[slot]);
+                    fold[SLOTS + slot] = __fmaf_rn(turned, above[b][k], turn == 0 ? 0.0f : fold[SLOTS + slot]);
+                    fold[2 * SLOTS + slot] = __fmaf_rn(turned, on[b][k], turn == 0 ? 0.0f : fold[2 * SLOTS + slot]);
+                }
+        }
         __syncthreads();
-        for (int c = threadIdx.x; c < 2 * I; c += THREADS) {
-            double s = red[c];
-            for (int k = 1; k < WAVES; ++k) s += red[k * 2 * I + c];
-            partial_bn[(size_t)blockIdx.x * 2 * I + c] = s;
+    }
+    float *p = partial + (size_t)blockIdx.x * (3 * SLOTS);
+    for (int slot = threadIdx.x; slot < 3 * SLOTS; slot += T8_THREADS) p[slot] = fold[slot];
+    const float s = turned * (sums + __shfl_xor(sums, 32, 64));
+    if (kh == 0) fold_sums[wave * 32 + n] = s;
+    __syncthreads();
+    if (threadIdx.x < 32 * NA) {
+        float t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < UNITS; ++k) t += fold_sums[(k * NA + threadIdx.x / 32) * 32 + threadIdx.x % 32];
+        partial_sums[(size_t)blockIdx.x * 64 + threadIdx.x] = t;
+    }
+}
+
+// Its workgroups added up in float64: grad_W, grad_b (blocks of their own) and, per 32 columns of g by
+// accumulator and lane half, the part of BatchNorm's column sums that its rows of W give: partial_bn
+// [32 NA][2][I].
+constexpr int T8_FOLD_SLOTS = 16, T8_FOLD_SLICES = 32;
+__global__ __launch_bounds__(T8_FOLD_SLOTS * T8_FOLD_SLICES) void tail8_fold_kernel(
+    const float *__restrict__ partial, const float *__restrict__ partial_sums, int nwg, int NA, int NI, int O, int I,
+    const float *__restrict__ W, L8Bn bn, float *__restrict__ grad_weight, float *__restrict__ grad_bias,
+    double *__restrict__ partial_bn)
+{
+    __shared__ double red[T8_FOLD_SLICES][4][T8_FOLD_SLOTS];
+    const int slot = threadIdx.x % T8_FOLD_SLOTS, slice = threadIdx.x / T8_FOLD_SLOTS;
+    const int slots = NA * NI * 1024, at = blockIdx.x * T8_FOLD_SLOTS + slot;
+    const bool of_bias = at >= slots;                       // (whole blocks)
+    const int lane = at & 63, e = (at >> 6) & 15, blk = at >> 10;
+    const int o = of_bias ? at - slots : blk / NI * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+    const int c = NI == 2 ? 2 * (lane & 31) + blk % 2 : lane & 31;
+    const int per = (nwg + T8_FOLD_SLICES - 1) / T8_FOLD_SLICES, k1 = min(nwg, (slice + 1) * per);
+    double s[4] = {0.0, 0.0, 0.0, 0.0};                     // of zq, on zq, on, g alone
+    if (of_bias) {
+        for (int k = slice * per; k < k1; ++k) s[3] += (double)partial_sums[(size_t)k * 64 + o];
+    } else {
+#pragma unroll 4
+        for (int k = slice * per; k < k1; ++k) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) s[i] += (double)partial[((size_t)k * 3 + i) * slots + at];
+            s[3] += (double)partial_sums[(size_t)k * 64 + o];
         }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[slice][i][slot] = s[i];
+    __syncthreads();
+    if (slice != 0) return;
+    for (int k = 1; k < T8_FOLD_SLICES; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] += red[k][i][slot];
+    if (of_bias) {
+        if (o < O) grad_bias[o] = (float)s[3];
+        return;
+    }
+    if (c >= I) return;
+    double P = 0.0, Q = 0.0, w = 0.0;
+    if (o < O) {
+        const double slope = (double)bn.slope;
+        P = slope * s[0] + (1.0 - slope) * s[1];            // (with the sign of gamma in it)
+        if (bn.weight && bn.weight[c] < 0.0f) P = -P;
+        Q = slope * s[3] + (1.0 - slope) * s[2];
+        w = (double)W[(size_t)o * I + c];
+        grad_weight[(size_t)o * I + c] =
+            (float)((bn.weight ? (double)bn.weight[c] : 1.0) * P + (bn.bias ? (double)bn.bias[c] : 0.0) * Q);
+    }
+    double *out = partial_bn + (size_t)((blk / NI * 16 + e) * 2 + (lane >> 5)) * 2 * I;
+    out[c] = o < O ? w * Q : 0.0;
+    out[I + c] = o < O ? w * P : 0.0;
 }
 
 static int l8_workgroups(i64 rows, int threads)
@@ -715,8 +868,7 @@ static void l8_forward(const float *x, int I, const float *W, const float *bias,
 // (the workgroups launched: the partial results there are)
 template <int MODE>
 static int l8_backward(const float *g, int O, const int8_t *codes, const uint8_t *exps, const float *W, int I, i64 rows,
-                        const L8Bn &bn, int want_sums, float *grad, float *partial, float *partial_sums, double *partial_bn,
-                        hipStream_t st)
+                        const L8Bn &bn, int want_sums, float *grad, float *partial, float *partial_sums, hipStream_t st)
 {
     int nwg = 0;
 #define MVF_L8B(KO_, KI_)                                                                                          \
@@ -725,10 +877,10 @@ static int l8_backward(const float *g, int O, const int8_t *codes, const uint8_t
         nwg = l8_workgroups(rows, threads);                                                                        \
         if (O == 8 * KO_)                                                                                          \
             hipLaunchKernelGGL((linear8_backward_kernel<KO_, KI_, MODE, true>), dim3((unsigned)nwg), dim3(threads), 0, st, \
-                               g, O, codes, exps, W, rows, bn, want_sums, grad, partial, partial_sums, partial_bn); \
+                               g, O, codes, exps, W, rows, bn, want_sums, grad, partial, partial_sums); \
         else                                                                                                       \
             hipLaunchKernelGGL((linear8_backward_kernel<KO_, KI_, MODE, false>), dim3((unsigned)nwg), dim3(threads), 0, st, \
-                               g, O, codes, exps, W, rows, bn, want_sums, grad, partial, partial_sums, partial_bn); \
+                               g, O, codes, exps, W, rows, bn, want_sums, grad, partial, partial_sums); \
     } while (0)
 #define MVF_L8B_KI(KO_)                                                                                            \
     do {                                                                                                           \
@@ -753,6 +905,42 @@ static void l8_fold(const float *partial, const float *partial_sums, int nwg, in
 {
     const int NA = O > 32 ? 2 : 1, NB = I > 32 ? 2 : 1;
     xty8_fold(partial, partial_sums, nwg, NA, NB, NA == 2, NB == 2, O, I, grad_weight, I, grad_bias, st);
+}
+
+// The sums' pass and its fold; the rows of partial_bn that hold BatchNorm's sums afterwards.
+static int l8_tail_sums(const float *g, int O, const int8_t *codes, const uint8_t *exps, const float *W, int I, i64 rows,
+                        const L8Bn &bn, float *grad_weight, float *grad_bias, float *partial, float *partial_sums,
+                        double *partial_bn, hipStream_t st)
+{
+    const int NA = O > 32 ? 2 : 1, NI = I > 32 ? 2 : 1, nwg = l8_workgroups(rows, T8_THREADS / NA);
+#define MVF_T8(KO_, KI_)                                                                                           \
+    do {                                                                                                           \
+        if (O == 8 * KO_)                                                                                          \
+            hipLaunchKernelGGL((tail8_sums_kernel<KO_, KI_, true>), dim3((unsigned)nwg), dim3(T8_THREADS), 0, st, g, O, codes, \
+                               exps, rows, bn, partial, partial_sums);                                             \
+        else                                                                                                       \
+            hipLaunchKernelGGL((tail8_sums_kernel<KO_, KI_, false>), dim3((unsigned)nwg), dim3(T8_THREADS), 0, st, g, O, codes, \
+                               exps, rows, bn, partial, partial_sums);                                             \
+    } while (0)
+#define MVF_T8_KI(KO_)                                                                                             \
+    do {                                                                                                           \
+        switch (I) {                                                                                               \
+        case 8: MVF_T8(KO_, 1); break;                                                                             \
+        case 16: MVF_T8(KO_, 2); break;                                                                            \
+        case 32: MVF_T8(KO_, 4); break;                                                                            \
+        default: MVF_T8(KO_, 8); break;                                                                            \
+        }                                                                                                          \
+    } while (0)
+    if (O <= 8) MVF_T8_KI(1);
+    else if (O <= 16) MVF_T8_KI(2);
+    else if (O <= 32) MVF_T8_KI(4);
+    else MVF_T8_KI(8);
+#undef MVF_T8_KI
+#undef MVF_T8
+    const int blocks = NA * NI * 1024 / T8_FOLD_SLOTS + (grad_bias ? 64 / T8_FOLD_SLOTS : 0);
+    hipLaunchKernelGGL(tail8_fold_kernel, dim3(blocks), dim3(T8_FOLD_SLOTS * T8_FOLD_SLICES), 0, st, (const float *)partial,
+                       (const float *)partial_sums, nwg, NA, NI, O, I, W, bn, grad_weight, grad_bias, partial_bn);
+    return 32 * NA;
 }
 
 static bool l8_aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
@@ -796,7 +984,7 @@ extern "C" int mvf_linear_rows8_backward(
     hipStream_t st = (hipStream_t)stream;
     float *partial = (float *)workspace, *partial_sums = (float *)((char *)workspace + mvf_xty_workspace_bytes());
     const int nwg = l8_backward<L8_LINEAR>(grad_y, O, codes, exps, weight, I, rows, L8Bn{}, grad_bias != nullptr, grad_x, partial,
-                                           partial_sums, nullptr, st);
+                                           partial_sums, st);
     l8_fold(partial, partial_sums, nwg, I, O, grad_weight, grad_bias, st);
     MVF_LAUNCH_CHECK();
     return MVF_OK;
@@ -855,12 +1043,11 @@ extern "C" int mvf_batch_norm_act_linear8_backward(
     char *xty = (char *)workspace + mvf_batch_norm_act8_workspace_bytes(I);
     float *partial = (float *)xty, *partial_sums = (float *)(xty + mvf_xty_workspace_bytes());
     const L8Bn bn = {nullptr, save_invstd, nullptr, bn_weight, bn_bias, w.terms, act, training, act ? slope : 1.0f};
-    const int nwg = l8_backward<L8_SUMS>(grad_y, O, codes, exps, weight, I, rows, bn, grad_bias != nullptr, nullptr, partial,
-                                         partial_sums, w.partial, st);
-    l8_fold(partial, partial_sums, nwg, I, O, grad_weight, grad_bias, st);
-    bn8_grad_terms(w, nwg, I, rows, grad_bn_weight, grad_bn_bias, st);
+    const int nblk = l8_tail_sums(grad_y, O, codes, exps, weight, I, rows, bn, grad_weight, grad_bias, partial, partial_sums,
+                                  w.partial, st);
+    bn8_grad_terms(w, nblk, I, rows, grad_bn_weight, grad_bn_bias, st);
     if (grad_z)
-        l8_backward<L8_APPLY>(grad_y, O, codes, exps, weight, I, rows, bn, 0, grad_z, nullptr, nullptr, nullptr, st);
+        l8_backward<L8_APPLY>(grad_y, O, codes, exps, weight, I, rows, bn, 0, grad_z, nullptr, nullptr, st);
     MVF_LAUNCH_CHECK();
     return MVF_OK;
 }

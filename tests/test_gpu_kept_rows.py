@@ -548,6 +548,53 @@ def test_two_steps_on_two_streams():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("I,O", [(64, 64), (64, 40), (16, 56), (32, 8), (8, 24), (33, 9)])
+@pytest.mark.parametrize("act", [True, False])
+def test_block_kinks_and_nan(I, O, act):
+    """Scales of both signs and zero, shifts that put whole columns on one side, rows of NaN and infinities
+    (eval mode), against the formulas on the same codes in float64.
+
+    A sum of 3000 rows is made of at most 6 matrix instructions a tile and 2 tiles a wave, each cutting
+    16 products and the sum off at a step of the largest (17 steps of 2 u), joined by 8 float32
+    additions and in float64: 12 * 34 + 8 < 512 u of the magnitudes."""
+    from mvfusion import packed, training as tr
+    rows = 3001
+    g = np.random.default_rng(I + O)
+    gamma, beta = g.normal(size=I), g.normal(size=I)
+    gamma[::5], gamma[3::7], beta[4::6] = 0.0, -gamma[3::7], 9.0 * np.sign(beta[4::6])
+    gamma, beta = gamma.astype(np.float32), beta.astype(np.float32)
+    z = rows_of(rows, I, 11)
+    z[5, 1], z[900, I - 1], z[rows - 1, 2] = np.nan, np.inf, -np.inf
+    bad = [1, I - 1, 2]
+    bn, lin = torch.nn.BatchNorm1d(I).cuda().eval(), torch.nn.Linear(I, O).cuda()
+    with torch.no_grad():
+        bn.weight.copy_(T(gamma))
+        bn.bias.copy_(T(beta))
+    slope = 0.25 if act else 1.0
+    x = T(z).cuda().requires_grad_(True)
+    gy = T(g.normal(size=(rows, O)).astype(np.float32)).cuda()
+    y = tr.batch_norm_act_linear(x, bn, torch.nn.LeakyReLU(slope), lin, keep="int8")
+    gx, dgamma, dbeta, dw, db = torch.autograd.grad(y, (x, bn.weight, bn.bias, lin.weight, lin.bias), gy)
+    _, codes, exps, invstd = tr._bn8_forward(x.detach(), bn.weight.detach(), bn.bias.detach(), bn.running_mean,
+                                             bn.running_var, bn.eps, slope, False, 0.0, None, None)
+    zq = packed.unpack_rows(codes, exps).double().cpu().numpy()
+    on = ref.bn_on(zq, gamma, beta)
+    t = np.where(on, 1.0, slope)
+    g64, w64 = gy.double().cpu().numpy(), lin.weight.detach().double().cpu().numpy()
+    gh = t * (g64 @ w64)
+    v = t * (gamma.astype(np.float64) * zq + beta)
+    good = np.setdiff1d(np.arange(I), bad)
+    within(dw.cpu().numpy()[:, good], (g64.T @ v)[:, good],
+           512 * U * (np.abs(g64).T @ (np.abs(gamma * zq) + np.abs(beta)))[:, good], "dw")
+    assert torch.isnan(dw[:, bad]).all() and torch.isnan(dgamma[bad]).all()
+    within(db.cpu().numpy(), g64.sum(0), 512 * U * np.abs(g64).sum(0), "db")
+    mag = np.abs(g64) @ np.abs(w64)
+    within(dbeta.cpu().numpy(), gh.sum(0), 512 * U * mag.sum(0), "dbeta")
+    within(dgamma.cpu().numpy()[good], (gh * zq).sum(0)[good], 512 * U * (mag * np.abs(zq)).sum(0)[good], "dgamma")
+    k = gamma.astype(np.float64) * invstd.cpu().double().numpy()
+    within(gx.cpu().numpy(), gh * k, 512 * U * mag * np.abs(k), "gx")
+
+
 @pytest.mark.parametrize("O", [64, 60])
 @pytest.mark.parametrize("tail", [False, True])
 def test_weight_gradient_has_no_common_shift(tail, O):
