@@ -567,9 +567,10 @@ int mvf_linear_rows8_backward(
 /* BatchNorm + LeakyReLU (mvf_batch_norm_act8_forward) and the Linear behind it in one pass over z (two
  * with batch statistics that no col_sums bring): the activated rows are never stored, and the codes are
  * all that the backward keeps of a row.  Shapes and alignment as for mvf_linear_rows8_*; y_sums /
- * n_y_sums: column sums of y (NULL: not wanted).  backward: two passes over grad_y and the codes,
- * grad_y W is formed in both and stored in none; grad_z, grad_bn_weight, grad_bn_bias and grad_bias may
- * be NULL.  workspace: mvf_batch_norm_act_linear8_workspace_bytes(I) in both directions. */
+ * n_y_sums: column sums of y (NULL: not wanted).  backward: two passes over grad_y and the codes, one of
+ * sums and one that writes grad_z; grad_y W is formed in the second and never stored.  grad_z,
+ * grad_bn_weight, grad_bn_bias and grad_bias may be NULL.  workspace:
+ * mvf_batch_norm_act_linear8_workspace_bytes(I) in both directions. */
 size_t mvf_batch_norm_act_linear8_workspace_bytes(int32_t I);
 int mvf_batch_norm_act_linear8_forward(
     const float *z, int64_t rows, int32_t I, const float *bn_weight, const float *bn_bias,
