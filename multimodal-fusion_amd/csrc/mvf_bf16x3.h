@@ -44,7 +44,8 @@ template <int PARTS> struct XtyParts {
 // The matrix cores add bf16 products to float32 sums by cutting off what does not fit, towards minus
 // infinity: over 2 M rows that shifts sums of zero-mean terms by 2e-6 of their typical size.  Odd
 // waves therefore sum the negated products (one operand's sign turned, by a factor or in its two
-// bf16) and are subtracted where waves are joined: the two halves' errors cancel.
+// bf16) and are subtracted where waves are joined: the two halves' errors cancel.  (Sums of terms of one
+// sign, which the same rounding makes shorter in every wave, end up to 6e-7 of themselves short at 2 M rows.)
 __device__ __forceinline__ float xty_turned(int wave) { return wave & 1 ? -1.0f : 1.0f; }
 __device__ __forceinline__ unsigned xty_flip(int wave) { return wave & 1 ? 0x80008000u : 0u; }
 

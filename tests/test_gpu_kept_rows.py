@@ -659,6 +659,24 @@ def test_more_than_2_31_values(op, I, O):
         assert float((a - b).abs().max()) <= 2 * last * U * float(mag)
 
 
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_block(reentrant):
+    """A block that is run again during the backward, on autograd's thread, sets the form itself."""
+    from torch.utils.checkpoint import checkpoint
+    from mvfusion import training as tr
+    lin, bn, act = torch.nn.Linear(64, 32).cuda(), torch.nn.BatchNorm1d(64).cuda().eval(), torch.nn.LeakyReLU(0.2)
+
+    def block(x):
+        with tr.keep_activations("int8"):
+            return tr.batch_norm_act_linear(x, bn, act, lin)
+    x = torch.randn(5000, 64, device="cuda", requires_grad=True)
+    params = [x, bn.weight, bn.bias, lin.weight, lin.bias]
+    gy = torch.randn(5000, 32, device="cuda")
+    want = torch.autograd.grad(block(x), params, gy)
+    checkpoint(block, x, use_reentrant=reentrant).backward(gy)
+    assert all(torch.equal(p.grad, w) for p, w in zip(params, want))
+
+
 def test_what_autograd_refuses():
     """No second derivative, and no parameter changed between forward and backward."""
     from mvfusion import training as tr

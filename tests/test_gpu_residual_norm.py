@@ -130,6 +130,15 @@ def test_shapes(rows, C, G, kind, keep):
     check(make(rows, C, kind, "layer" if C > 1 else "rms", "rms", G, True, C % 3 == 0), kind, keep)
 
 
+# every team of lanes, with whole pieces of 16 bytes and with every size of a cut one
+@pytest.mark.parametrize("keep", ["float32", "int8"])
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("C", [16, 24, 27, 61, 64, 94, 96, 125, 183, 190, 192, 253, 382, 384, 511, 760, 767, 1022, 1024, 1049,
+                               1528, 1534, 2042, 2045])
+def test_teams(C, kind, keep):
+    check(make(37, C, kind, "rms", "layer", 1, True, True), kind, keep)
+
+
 @pytest.mark.parametrize("keep", ["float32", "int8"])
 @pytest.mark.parametrize("kind,rows,C,G", [("float32", 20003, 64, 4), ("bfloat16", 3001, 512, 1), ("float16", 40001, 24, 2)])
 def test_many_rows(kind, rows, C, G, keep):
@@ -311,6 +320,22 @@ def test_same_bits_other_streams_and_replays():
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
+@pytest.mark.parametrize("keep", ["float32", "int8"])
+def test_one_tensor_on_both_sides(keep):
+    """f the tensor x itself, one norm on both sides: the sums of what two of each get."""
+    from mvfusion.residual import residual_norm
+    torch.manual_seed(2)
+    x = torch.randn(300, 48, device="cuda", requires_grad=True)
+    f = x.detach().clone().requires_grad_(True)
+    m, m2 = torch.nn.LayerNorm(48).cuda(), torch.nn.LayerNorm(48).cuda()
+    d = torch.randn(2, 300, 48, device="cuda")
+    one = torch.autograd.grad(residual_norm(x, x, post=m, pre=m, keep=keep), (x, m.weight, m.bias), list(d))
+    two = torch.autograd.grad(residual_norm(x, f, post=m2, pre=m, keep=keep),
+                              (x, f, m2.weight, m.weight, m2.bias, m.bias), list(d))
+    for k in range(3):
+        assert torch.equal(one[k], two[2 * k] + two[2 * k + 1])
 
 
 def test_more_than_2_31_values():
