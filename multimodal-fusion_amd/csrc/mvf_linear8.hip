@@ -420,7 +420,8 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
         int e[KI];
 #pragma unroll
         for (int j = 0; j < KI; ++j) {
-            q[j] = qw[j];
+            // (rows past the end as zeros here too: a code of NaN would survive the zeros of g)
+            q[j] = WHOLE || row0 + j * (64 / IQ) < live ? qw[j] : 0u;
             e[j] = __shfl(ew, (row0 + j * (64 / IQ)) * GR + col / R8_GROUP, 64);
             if constexpr (XTY) {
                 float v[4];
@@ -671,6 +672,8 @@ __global__ __launch_bounds__(T8_THREADS) void tail8_sums_kernel(
         float least = 0.0f;
 #pragma unroll
         for (int j = 0; j < KI; ++j) {
+            // (rows past the end as zeros here too: a code of NaN would survive the zeros of g)
+            if (!WHOLE && row0 + j * (64 / IQ) >= live) qw[j] = 0u;
             e[j] = __shfl(ew, (row0 + j * (64 / IQ)) * GR + col / R8_GROUP, 64);
             const float step = ldexpf(1.0f, e[j] - R8_BIAS);
             float c[4];

@@ -1,0 +1,90 @@
+"""Kept rows at the edges of what is documented: values that are not finite next to the end of the rows,
+modules whose parameters are made on the fly, kinks at the end of the codes' range, rows and layers that
+do not fit, no rows, long sums of one sign.
+
+Tolerances as in test_gpu_kept_rows: u = 2^-24 per float32 operation, times the sum of magnitudes."""
+import numpy as np
+import pytest
+import torch
+
+import kept_rows_reference as ref
+import test_gpu_kept_rows as base
+
+pytestmark = pytest.mark.gpu
+U = base.U
+T = base.T
+within = base.within
+
+
+# ---- a value that is not finite in the last, cut tile -----------------------------------------------
+SHAPES = [(64, 64), (64, 40), (32, 8), (16, 56), (8, 24), (33, 9)]
+
+
+@pytest.mark.parametrize("I,O", SHAPES)
+@pytest.mark.parametrize("rows", [5, 3001])
+def test_linear_nan_in_the_last_row(rows, I, O):
+    """The last value of the last row is NaN, the one three columns before it infinite: their columns of
+    the weight gradient are NaN, and no others (the lanes past the last row must not bring them back)."""
+    from mvfusion import training as tr
+    g = np.random.default_rng(rows + I)
+    lin = torch.nn.Linear(I, O).cuda()
+    x = g.normal(size=(rows, I)).astype(np.float32)
+    x[rows - 1, I - 1], x[rows - 1, I - 4] = np.nan, np.inf
+    bad = [I - 4, I - 1]
+    gy = g.normal(size=(rows, O)).astype(np.float32)
+    xt = T(x).cuda().requires_grad_(True)
+    y = tr.linear(lin, xt, keep="int8")
+    gx, gw, gb = (t.cpu().numpy() for t in torch.autograd.grad(y, (xt, lin.weight, lin.bias), T(gy).cuda()))
+    good = np.setdiff1d(np.arange(I), bad)
+    xq = ref.unpack(*ref.pack(x))[:, good]
+    g64, w64 = gy.astype(np.float64), lin.weight.detach().cpu().double().numpy()
+    within(gw[:, good], g64.T @ xq, base.xty_bound(g64, xq, rows), "weight")
+    assert np.isnan(gw[:, bad]).all()
+    within(gx, g64 @ w64, (O + 2) * U * (np.abs(g64) @ np.abs(w64)), "x")
+    within(gb, g64.sum(0), 64 * U * np.abs(g64).sum(0), "bias")
+
+
+@pytest.mark.parametrize("training", [False, True])
+@pytest.mark.parametrize("I,O", SHAPES)
+def test_block_nan_in_the_last_row(I, O, training):
+    """The same behind BatchNorm: in train mode the statistics make the whole column NaN, and only it.
+    512 u: the sums of 3000 rows as in test_block_kinks_and_nan."""
+    from mvfusion import packed, training as tr
+    rows = 3001
+    g = np.random.default_rng(I + O)
+    bn, lin = torch.nn.BatchNorm1d(I).cuda().train(training), torch.nn.Linear(I, O).cuda()
+    gamma, beta = (1 + 0.3 * g.normal(size=I)).astype(np.float32), (0.3 * g.normal(size=I)).astype(np.float32)
+    with torch.no_grad():
+        bn.weight.copy_(T(gamma))
+        bn.bias.copy_(T(beta))
+    z = base.rows_of(rows, I, 11)
+    z[rows - 1, I - 1] = np.nan
+    x = T(z).cuda().requires_grad_(True)
+    gy = T(g.normal(size=(rows, O)).astype(np.float32)).cuda()
+    state = {k: v.clone() for k, v in bn.state_dict().items()}
+    y = tr.batch_norm_act_linear(x, bn, torch.nn.LeakyReLU(0.25), lin, keep="int8")
+    gx, dgamma, dbeta, dw = (t.cpu().numpy() for t in
+                             torch.autograd.grad(y, (x, bn.weight, bn.bias, lin.weight), gy))
+    bn.load_state_dict(state)
+    _, codes, exps, invstd = tr._bn8_forward(x.detach(), bn.weight.detach(), bn.bias.detach(), bn.running_mean,
+                                             bn.running_var, bn.eps, 0.25, training, 0.1, None, None)
+    zq = packed.unpack_rows(codes, exps).double().cpu().numpy()
+    good = np.arange(I - 1)
+    t = np.where(ref.bn_on(zq, gamma, beta), 1.0, 0.25)
+    g64, w64 = gy.double().cpu().numpy(), lin.weight.detach().double().cpu().numpy()
+    gh, mag = (t * (g64 @ w64))[:, good], (np.abs(g64) @ np.abs(w64))[:, good]
+    v = (t * (gamma.astype(np.float64) * zq + beta))[:, good]
+    zq = zq[:, good]
+    vmag = np.abs(gamma[good] * zq) + np.abs(beta[good])
+    within(dw[:, good], g64.T @ v, 512 * U * (np.abs(g64).T @ vmag), "dw")
+    assert np.isnan(dw[:, I - 1]).all() and np.isnan(dgamma[I - 1])
+    within(dbeta[good], gh.sum(0), 512 * U * mag.sum(0), "dbeta")
+    within(dgamma[good], (gh * zq).sum(0), 512 * U * (mag * np.abs(zq)).sum(0), "dgamma")
+    k = (gamma.astype(np.float64) * invstd.cpu().double().numpy())[good]
+    if training:
+        want = (gh - gh.mean(0) - zq * (gh * zq).mean(0)) * k
+        mag = mag + mag.mean(0) + np.abs(zq) * (mag * np.abs(zq)).mean(0)
+    else:
+        want = gh * k
+        assert np.isfinite(gx).all()
+    within(gx[:, good], want, 512 * U * mag * np.abs(k), "gx")
