@@ -308,13 +308,17 @@ class _BatchNormActLinear8(torch.autograd.Function):
         return (gz, gw, gb, glw, glb) + (None,) * 9
 
 
+def _takes_bn(z, bn):
+    return (z.is_cuda and z.dtype == torch.float32 and z.dim() == 2 and z.shape[0] > 0
+            and isinstance(bn, torch.nn.BatchNorm1d))
+
+
 def _bn_plan(z, bn, kernel_counts=False):
     """(running mean, running variance, batch_stats, factor, counter) of an nn.BatchNorm1d's next
     call on z; None where this package's kernels do not take z or the module.  The batch is
     counted in num_batches_tracked here, or, with kernel_counts, by the kernel that is given
     the counter (None: already counted, or nothing to count)."""
-    if not (z.is_cuda and z.dtype == torch.float32 and z.dim() == 2 and z.shape[0] > 0
-            and isinstance(bn, torch.nn.BatchNorm1d)):
+    if not _takes_bn(z, bn):
         return None
     weight, bias = bn._parameters["weight"], bn._parameters["bias"]
     rm, rv, tracked = (bn._buffers.get(k) for k in ("running_mean", "running_var", "num_batches_tracked"))
@@ -350,7 +354,8 @@ def batch_norm_act(z, bn, act, col_sums=None, keep=None):
     (a value that is not finite then counts as not above the activation's kink);
     None: as ``keep_activations`` says."""
     fused_act = isinstance(act, torch.nn.LeakyReLU)
-    keeps8 = _keeps8(keep, z, bn.weight, bn.bias)
+    kept_form(keep)
+    keeps8 = _takes_bn(z, bn) and _keeps8(keep, z, bn.weight, bn.bias)
     plan = _bn_plan(z, bn, keeps8)
     if plan is None:
         return act(bn(z))
@@ -368,7 +373,7 @@ def batch_norm_act_linear(z, bn, act, lin, col_sums=None, want_sums=False, keep=
     """``linear(lin, batch_norm_act(z, bn, act, col_sums), want_sums)``.  With 'int8'
     rows (``keep``, ``keep_activations``) and a LeakyReLU the two keep one packed copy
     of the normalised rows between them; elsewhere they are two calls."""
-    if (isinstance(act, torch.nn.LeakyReLU) and _takes(lin, z)
+    if (isinstance(act, torch.nn.LeakyReLU) and _takes(lin, z) and _takes_bn(z, bn)
             and _keeps8(keep, z, bn.weight, bn.bias, lin.weight, lin.bias)):
         plan = _bn_plan(z, bn, True)
         if plan is not None:
