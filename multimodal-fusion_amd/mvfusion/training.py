@@ -313,15 +313,12 @@ def _takes_bn(z, bn):
             and isinstance(bn, torch.nn.BatchNorm1d))
 
 
-def _bn_plan(z, bn, kernel_counts=False):
-    """(running mean, running variance, batch_stats, factor, counter) of an nn.BatchNorm1d's next
-    call on z; None where this package's kernels do not take z or the module.  The batch is
-    counted in num_batches_tracked here, or, with kernel_counts, by the kernel that is given
-    the counter (None: already counted, or nothing to count)."""
-    if not _takes_bn(z, bn):
-        return None
-    weight, bias = bn._parameters["weight"], bn._parameters["bias"]
-    rm, rv, tracked = (bn._buffers.get(k) for k in ("running_mean", "running_var", "num_batches_tracked"))
+def _bn_plan(z, bn, weight, bias, kernel_counts=False):
+    """(running mean, running variance, batch_stats, factor, counter) of the next call on z of an
+    nn.BatchNorm1d with these parameters; None where this package's kernels do not take one of its
+    tensors.  The batch is counted in num_batches_tracked here, or, with kernel_counts, by the kernel
+    that is given the counter (None: already counted, or nothing to count)."""
+    rm, rv, tracked = bn.running_mean, bn.running_var, bn.num_batches_tracked
     for t in (weight, bias, rm, rv):
         if t is not None and not (t.device == z.device and t.dtype == torch.float32):
             return None
@@ -355,17 +352,20 @@ def batch_norm_act(z, bn, act, col_sums=None, keep=None):
     None: as ``keep_activations`` says."""
     fused_act = isinstance(act, torch.nn.LeakyReLU)
     kept_form(keep)
-    keeps8 = _takes_bn(z, bn) and _keeps8(keep, z, bn.weight, bn.bias)
-    plan = _bn_plan(z, bn, keeps8)
+    if not _takes_bn(z, bn):
+        return act(bn(z))
+    weight, bias = bn.weight, bn.bias
+    keeps8 = _keeps8(keep, z, weight, bias)
+    plan = _bn_plan(z, bn, weight, bias, keeps8)
     if plan is None:
         return act(bn(z))
     rm, rv, batch_stats, factor, counter = plan
     slope = float(act.negative_slope) if fused_act else None
     col_sums = col_sums if batch_stats else None
     if keeps8:
-        y = _BatchNormAct8.apply(z, bn.weight, bn.bias, rm, rv, bn.eps, slope, batch_stats, factor, counter, col_sums)
+        y = _BatchNormAct8.apply(z, weight, bias, rm, rv, bn.eps, slope, batch_stats, factor, counter, col_sums)
     else:
-        y = _BatchNormAct.apply(z, bn.weight, bn.bias, rm, rv, bn.eps, slope, batch_stats, factor, col_sums)
+        y = _BatchNormAct.apply(z, weight, bias, rm, rv, bn.eps, slope, batch_stats, factor, col_sums)
     return y if fused_act else act(y)
 
 
@@ -373,15 +373,16 @@ def batch_norm_act_linear(z, bn, act, lin, col_sums=None, want_sums=False, keep=
     """``linear(lin, batch_norm_act(z, bn, act, col_sums), want_sums)``.  With 'int8'
     rows (``keep``, ``keep_activations``) and a LeakyReLU the two keep one packed copy
     of the normalised rows between them; elsewhere they are two calls."""
-    if (isinstance(act, torch.nn.LeakyReLU) and _takes(lin, z) and _takes_bn(z, bn)
-            and _keeps8(keep, z, bn.weight, bn.bias, lin.weight, lin.bias)):
-        plan = _bn_plan(z, bn, True)
-        if plan is not None:
-            rm, rv, batch_stats, factor, counter = plan
-            y, sums = _BatchNormActLinear8.apply(
-                z, bn.weight, bn.bias, lin.weight, lin.bias, rm, rv, bn.eps, float(act.negative_slope),
-                batch_stats, factor, counter, col_sums if batch_stats else None, bool(want_sums))
-            return (y, sums) if want_sums else y
+    if isinstance(act, torch.nn.LeakyReLU) and _takes(lin, z) and _takes_bn(z, bn):
+        weight, bias = bn.weight, bn.bias
+        if _keeps8(keep, z, weight, bias, lin.weight, lin.bias):
+            plan = _bn_plan(z, bn, weight, bias, True)
+            if plan is not None:
+                rm, rv, batch_stats, factor, counter = plan
+                y, sums = _BatchNormActLinear8.apply(
+                    z, weight, bias, lin.weight, lin.bias, rm, rv, bn.eps, float(act.negative_slope),
+                    batch_stats, factor, counter, col_sums if batch_stats else None, bool(want_sums))
+                return (y, sums) if want_sums else y
     form = {} if keep is None else {"keep": keep}
     return linear(lin, batch_norm_act(z, bn, act, col_sums=col_sums, **form), want_sums, **form)
 

@@ -6,6 +6,7 @@ Tolerances as in test_gpu_kept_rows: u = 2^-24 per float32 operation, times the 
 import numpy as np
 import pytest
 import torch
+from torch.nn.utils import parametrize, prune
 
 import kept_rows_reference as ref
 import test_gpu_kept_rows as base
@@ -88,3 +89,50 @@ def test_block_nan_in_the_last_row(I, O, training):
         want = gh * k
         assert np.isfinite(gx).all()
     within(gx[:, good], want, 512 * U * mag * np.abs(k), "gx")
+
+
+# ---- parameters that are made on the fly -------------------------------------------------------------
+class Doubled(torch.nn.Module):
+    def forward(self, w):
+        return 2 * w
+
+
+def made(bn, how):
+    """bn with a weight that is no entry of its own parameters."""
+    if how == "parametrized":
+        parametrize.register_parametrization(bn, "weight", Doubled())
+    elif how == "pruned":
+        prune.random_unstructured(bn, "weight", 0.5)
+    elif how == "replica":
+        (bn,) = torch.nn.parallel.replicate(bn, [0])
+    return bn
+
+
+@pytest.mark.parametrize("keep", ["float32", "int8"])
+@pytest.mark.parametrize("how", ["parametrized", "pruned", "replica"])
+def test_batch_norm_with_a_made_weight(how, keep):
+    """The kernels take a BatchNorm whose weight is parametrized, pruned or a replica's copy: what a plain
+    module with the same weight gives, and the gradient of the parameter underneath."""
+    from mvfusion import training as tr
+    torch.manual_seed(4)
+    source, act, lin = torch.nn.BatchNorm1d(40).cuda(), torch.nn.LeakyReLU(0.2), torch.nn.Linear(40, 8).cuda()
+    with torch.no_grad():
+        source.weight.uniform_(0.5, 2)
+        source.bias.uniform_(-1, 1)
+    bn = made(source, how)
+    plain = torch.nn.BatchNorm1d(40).cuda()
+    with torch.no_grad():
+        plain.weight.copy_(bn.weight)
+        plain.bias.copy_(bn.bias)
+    x, gy = torch.randn(5000, 40, device="cuda", requires_grad=True), torch.randn(5000, 40, device="cuda")
+    under = next(p for n, p in source.named_parameters() if "weight" in n)
+    (factor,) = torch.autograd.grad(bn.weight.sum(), under, retain_graph=True)
+    y, want = tr.batch_norm_act(x, bn, act, keep=keep), tr.batch_norm_act(x, plain, act, keep=keep)
+    assert torch.equal(y, want)
+    gx, gw = torch.autograd.grad(y, (x, under), gy, retain_graph=True)   # (pruning makes the weight once)
+    wx, ww = torch.autograd.grad(want, (x, plain.weight), gy)
+    assert torch.equal(gx, wx) and torch.equal(gw, ww * factor)
+    assert torch.equal(bn.running_mean, plain.running_mean) and int(bn.num_batches_tracked) == 1
+    y, want = tr.batch_norm_act_linear(x, bn, act, lin, keep=keep), tr.batch_norm_act_linear(x, plain, act, lin, keep=keep)
+    assert torch.equal(y, want)
+    assert torch.equal(torch.autograd.grad(y, x, gy[:, :8])[0], torch.autograd.grad(want, x, gy[:, :8])[0])
