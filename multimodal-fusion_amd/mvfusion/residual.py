@@ -20,7 +20,8 @@ _NONE, _RMS, _LAYER = 0, 1, 2
 
 
 def _norm_args(norm, C, x, name):
-    """(kind, weight, bias, eps) of an nn.RMSNorm / nn.LayerNorm over the channels."""
+    """(kind, weight, bias, eps) of an nn.RMSNorm / nn.LayerNorm over the channels (attributes: a
+    parametrized or replicated weight is no entry of the module's own parameters)."""
     if norm is None:
         return _NONE, None, None, 0.0
     if isinstance(norm, torch.nn.LayerNorm):
@@ -32,8 +33,7 @@ def _norm_args(norm, C, x, name):
     if tuple(norm.normalized_shape) != (C,):
         raise ValueError(f"residual_norm: {name} normalises {tuple(norm.normalized_shape)}, the rows have {C} channels")
     eps = torch.finfo(x.dtype).eps if norm.eps is None else float(norm.eps)
-    params = norm._parameters
-    return kind, _vector(params["weight"], C, x, name), _vector(params.get("bias"), C, x, name), eps
+    return kind, _vector(norm.weight, C, x, name), _vector(getattr(norm, "bias", None), C, x, name), eps
 
 
 def _vector(t, C, x, name):
@@ -122,7 +122,8 @@ def residual_norm(x, f, post=None, pre=None, gate=None, scale=None, seen=None, k
     :param x: [..., C] float32, bfloat16 or float16 rows on the HIP device, C <= 4096
     :param f: rows like x, the branch's output; None: out = x (the norm in front of
         the first branch)
-    :param post, pre: nn.RMSNorm or nn.LayerNorm over the C channels, or None
+    :param post, pre: nn.RMSNorm or nn.LayerNorm over the C channels, or None; their weights,
+        biases and eps are read, the modules are not called (hooks on them do not run)
     :param gate: [...] or [..., G] with C % G == 0, G groups of neighbouring channels
     :param scale: [C], one element, or a number
     :param seen: [...] bool; where False nothing is added and f is not read, so

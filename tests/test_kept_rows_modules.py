@@ -1,8 +1,9 @@
 """Which modules the training path's layers accept, without a GPU."""
 import pytest
 import torch
+from torch.nn.utils import parametrize, prune
 
-from mvfusion import training
+from mvfusion import residual, training
 
 
 @pytest.mark.parametrize("keep", [None, "float32", "int8"])
@@ -21,3 +22,27 @@ def test_other_modules_in_place_of_the_norm(norm, keep):
         training.batch_norm_act(x, norm, act, keep="bits")
     with pytest.raises(ValueError):
         training.batch_norm_act_linear(x, norm, act, lin, keep="bits")
+
+
+class Doubled(torch.nn.Module):
+    def forward(self, w):
+        return 2 * w
+
+
+def test_residual_norms_with_made_weights():
+    """The norms' parameters are read as attributes: parametrized and pruned ones, and none at all."""
+    rows = torch.zeros(3, 8)
+    norm = torch.nn.LayerNorm(8, eps=1e-3)
+    parametrize.register_parametrization(norm, "weight", Doubled())
+    prune.random_unstructured(norm, "bias", 0.5)
+    kind, weight, bias, eps = residual._norm_args(norm, 8, rows, "post")
+    assert kind == residual._LAYER and eps == 1e-3
+    assert torch.equal(weight, 2 * torch.ones(8)) and weight.requires_grad and torch.equal(bias, norm.bias)
+    rms = torch.nn.RMSNorm(8)
+    parametrize.register_parametrization(rms, "weight", Doubled())
+    kind, weight, bias, eps = residual._norm_args(rms, 8, rows, "pre")
+    assert kind == residual._RMS and bias is None and eps == torch.finfo(torch.float32).eps
+    assert torch.equal(weight, 2 * torch.ones(8))
+    for none in (torch.nn.LayerNorm(8, elementwise_affine=False), torch.nn.RMSNorm(8, elementwise_affine=False)):
+        assert residual._norm_args(none, 8, rows, "pre")[1:3] == (None, None)
+    assert residual._norm_args(torch.nn.LayerNorm(8, bias=False), 8, rows, "pre")[2] is None
