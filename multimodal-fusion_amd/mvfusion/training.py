@@ -598,6 +598,8 @@ def mlp_on_rows_and_sets(seq, x, x_set, ptr):
     (DeepSetFeat's 'concatenation' fusion, pooling.py:669-681)."""
     lin = seq[0][0]
     d = x.shape[1]
+    if x.shape[0] == 0:
+        return mlp(seq, torch.cat((x, P.gather_csr(x_set, ptr)), dim=1))
     za = _linear(x, lin.weight[:, :d], None)[0]
     zb = _linear(x_set, lin.weight[:, d:], lin.bias)[0]
     return _mlp_tail(seq, za + P.gather_csr(zb, ptr))

@@ -136,3 +136,37 @@ def test_batch_norm_with_a_made_weight(how, keep):
     y, want = tr.batch_norm_act_linear(x, bn, act, lin, keep=keep), tr.batch_norm_act_linear(x, plain, act, lin, keep=keep)
     assert torch.equal(y, want)
     assert torch.equal(torch.autograd.grad(y, x, gy[:, :8])[0], torch.autograd.grad(want, x, gy[:, :8])[0])
+
+
+# ---- no rows ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("keep", ["float32", "int8"])
+def test_pool_of_points_without_views(keep):
+    """A sample none of whose points has a view, in eval mode with a graph: zeros, and zero gradients of
+    whatever the views go through."""
+    from mvfusion import training as tr
+    pool = base.make_pool().eval()
+    x = [torch.randn(s, device="cuda", requires_grad=True) for s in ((7, 24), (0, 64), (0, 8))]
+    ptr = torch.zeros(8, dtype=torch.int64, device="cuda")
+    with tr.keep_activations(keep):
+        out = pool(x[0], x[1], x[2], ptr)
+    assert out.shape == (7, 64) and not out.any()
+    grads = torch.autograd.grad(out.sum(), x + list(pool.parameters()), allow_unused=True)
+    assert all(g is None or not g.any() for g in grads)
+
+
+@pytest.mark.parametrize("keep", ["float32", "int8"])
+def test_layers_without_rows(keep):
+    """Every layer of the training path on no rows, in eval mode."""
+    from mvfusion import training as tr
+    from mvfusion.dense import MLP
+    lin, bn, act = torch.nn.Linear(64, 32).cuda(), torch.nn.BatchNorm1d(64).cuda().eval(), torch.nn.LeakyReLU(0.2)
+    seq = MLP([40 + 24, 32, 16], bias=False).cuda().eval()
+    x = torch.empty(0, 64, device="cuda", requires_grad=True)
+    ptr = torch.zeros(5, dtype=torch.int64, device="cuda")
+    with tr.keep_activations(keep):
+        assert tr.linear(lin, x).shape == (0, 32) and tr.batch_norm_act(x, bn, act).shape == (0, 64)
+        assert tr.batch_norm_act_linear(x, bn, act, lin).shape == (0, 32) and tr.mlp(seq, x).shape == (0, 16)
+        y = tr.mlp_on_rows_and_sets(seq, x[:, :40], torch.randn(4, 24, device="cuda"), ptr)
+        assert y.shape == (0, 16)
+    (gw,) = torch.autograd.grad(y.sum(), seq[0][0].weight)
+    assert gw.shape == (32, 64) and not gw.any()
