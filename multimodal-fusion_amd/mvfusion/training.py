@@ -310,7 +310,7 @@ class _BatchNormActLinear8(torch.autograd.Function):
 
 def _takes_bn(z, bn):
     return (z.is_cuda and z.dtype == torch.float32 and z.dim() == 2 and z.shape[0] > 0
-            and isinstance(bn, torch.nn.BatchNorm1d))
+            and isinstance(bn, torch.nn.BatchNorm1d) and z.shape[1] == bn.num_features)
 
 
 def _bn_plan(z, bn, weight, bias, kernel_counts=False):
@@ -320,7 +320,7 @@ def _bn_plan(z, bn, weight, bias, kernel_counts=False):
     that is given the counter (None: already counted, or nothing to count)."""
     rm, rv, tracked = bn.running_mean, bn.running_var, bn.num_batches_tracked
     for t in (weight, bias, rm, rv):
-        if t is not None and not (t.device == z.device and t.dtype == torch.float32):
+        if t is not None and not (t.device == z.device and t.dtype == torch.float32 and t.shape == z.shape[1:]):
             return None
     batch_stats = bn.training or rm is None
     factor, counter = 0.0, None
@@ -536,9 +536,16 @@ class _Linear8(torch.autograd.Function):
         return gx, gw, gb, None
 
 
-def _takes(lin, x):
+def _fits(x, weight, bias):
+    """Can the kernels take rows x through this Linear?  (They read as many columns as the weight has,
+    and parameters as float32 on the device of the rows.)"""
     return (x.is_cuda and x.dtype == torch.float32 and x.dim() == 2 and x.shape[0] > 0
-            and lin.weight.device == x.device and lin.weight.dtype == torch.float32)
+            and weight.device == x.device and weight.dtype == torch.float32 and weight.shape[1] == x.shape[1]
+            and (bias is None or (bias.device == x.device and bias.dtype == torch.float32)))
+
+
+def _takes(lin, x):
+    return _fits(x, lin.weight, lin.bias)
 
 
 def _linear(x, weight, bias, want_sums=False, keep=None):
@@ -598,10 +605,11 @@ def mlp_on_rows_and_sets(seq, x, x_set, ptr):
     (DeepSetFeat's 'concatenation' fusion, pooling.py:669-681)."""
     lin = seq[0][0]
     d = x.shape[1]
-    if x.shape[0] == 0:
+    wa, wb = lin.weight[:, :d], lin.weight[:, d:]
+    if not (_fits(x, wa, None) and _fits(x_set, wb, lin.bias)):
         return mlp(seq, torch.cat((x, P.gather_csr(x_set, ptr)), dim=1))
-    za = _linear(x, lin.weight[:, :d], None)[0]
-    zb = _linear(x_set, lin.weight[:, d:], lin.bias)[0]
+    za = _linear(x, wa, None)[0]
+    zb = _linear(x_set, wb, lin.bias)[0]
     return _mlp_tail(seq, za + P.gather_csr(zb, ptr))
 
 

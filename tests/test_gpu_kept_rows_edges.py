@@ -170,3 +170,41 @@ def test_layers_without_rows(keep):
         assert y.shape == (0, 16)
     (gw,) = torch.autograd.grad(y.sum(), seq[0][0].weight)
     assert gw.shape == (32, 64) and not gw.any()
+
+
+# ---- layers that do not fit the rows ------------------------------------------------------------------
+@pytest.mark.parametrize("keep", ["float32", "int8"])
+@pytest.mark.parametrize("rows", [40, 5000])
+def test_widths_that_do_not_fit(rows, keep):
+    """A layer of another width than the rows is the module's to refuse: no kernel runs on it."""
+    from mvfusion import _lib, training as tr
+    x = torch.randn(rows, 32, device="cuda", requires_grad=True)
+    act, bn = torch.nn.LeakyReLU(0.2), torch.nn.BatchNorm1d(32).cuda()
+    for width in (16, 64):
+        lin, other = torch.nn.Linear(width, 8).cuda(), torch.nn.BatchNorm1d(width).cuda()
+        for call in (lambda: tr.linear(lin, x, keep=keep), lambda: tr.batch_norm_act(x, other, act, keep=keep),
+                     lambda: tr.batch_norm_act_linear(x, bn, act, lin, keep=keep),
+                     lambda: tr.batch_norm_act_linear(x, other, act, torch.nn.Linear(32, 8).cuda(), keep=keep),
+                     lambda: tr.linear(lin.cpu(), x, keep=keep)):
+            with pytest.raises(RuntimeError) as e:
+                call()
+            assert not isinstance(e.value, _lib.MvfError)
+
+
+@pytest.mark.parametrize("keep", ["float32", "int8"])
+def test_sets_that_do_not_fit(keep):
+    """The split first Linear of the set encoder: the halves have to fit rows and sets, and parameters on
+    the host are refused rather than read."""
+    from mvfusion import training as tr
+    from mvfusion.dense import MLP
+    seq = MLP([64, 32, 16], bias=False).cuda().eval()
+    ptr = torch.tensor([0, 3, 3, 20], device="cuda")
+    x, sets = torch.randn(20, 32, device="cuda", requires_grad=True), torch.randn(3, 32, device="cuda")
+    with tr.keep_activations(keep):
+        want = tr.mlp(seq, torch.cat((x, sets.repeat_interleave(ptr.diff(), dim=0)), 1))
+        assert torch.allclose(tr.mlp_on_rows_and_sets(seq, x, sets, ptr), want, rtol=1e-5, atol=1e-5)
+        for bad in ((x, sets[:, :16]), (x[:, :16], sets), (x, torch.randn(3, 48, device="cuda"))):
+            with pytest.raises(RuntimeError):
+                tr.mlp_on_rows_and_sets(seq, *bad, ptr)
+        with pytest.raises(RuntimeError):
+            tr.mlp_on_rows_and_sets(seq.cpu(), x, sets, ptr)

@@ -46,3 +46,30 @@ def test_residual_norms_with_made_weights():
     for none in (torch.nn.LayerNorm(8, elementwise_affine=False), torch.nn.RMSNorm(8, elementwise_affine=False)):
         assert residual._norm_args(none, 8, rows, "pre")[1:3] == (None, None)
     assert residual._norm_args(torch.nn.LayerNorm(8, bias=False), 8, rows, "pre")[2] is None
+
+
+class Rows:
+    """Rows as the choice of a kernel sees them: on a device, without values."""
+
+    def __init__(self, *shape, dtype=torch.float32, device="cuda:0"):
+        self.shape, self.dtype, self.device, self.is_cuda = torch.Size(shape), dtype, torch.device(device), True
+
+    def dim(self):
+        return len(self.shape)
+
+
+def test_kernels_are_chosen_by_width_type_and_device():
+    x, w = Rows(5, 32), Rows(8, 32)
+    assert training._fits(x, w, None) and training._fits(x, w, Rows(8))
+    for bad in (Rows(8, 16), Rows(8, 64), Rows(8, 32, dtype=torch.float16), Rows(8, 32, device="cuda:1"), torch.zeros(8, 32)):
+        assert not training._fits(x, bad, None)
+    for bias in (Rows(8, dtype=torch.float16), Rows(8, device="cuda:1"), torch.zeros(8)):
+        assert not training._fits(x, w, bias)
+    for rows in (Rows(0, 32), Rows(5, 2, 32), Rows(5, 32, dtype=torch.float64)):
+        assert not training._fits(rows, w, None)
+    assert training._takes_bn(x, torch.nn.BatchNorm1d(32)) and not training._takes_bn(x, torch.nn.BatchNorm1d(16))
+    assert not training._takes_bn(Rows(0, 32), torch.nn.BatchNorm1d(32))
+    host, bn = Rows(5, 32, device="cpu"), torch.nn.BatchNorm1d(32).eval()
+    assert training._bn_plan(host, bn, bn.weight, bn.bias) is not None
+    bn.running_mean = torch.zeros(16)
+    assert training._bn_plan(host, bn, bn.weight, bn.bias) is None
