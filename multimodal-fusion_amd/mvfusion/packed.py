@@ -55,6 +55,13 @@ def _check_rows(x, what):
         raise TypeError(f"mvfusion {what} expects float32, bfloat16 or float16 rows, got {x.dtype}")
 
 
+def check_codes(codes, exps, what):
+    """Refuses what is not the two parts of 8-bit rows."""
+    if (codes.dtype != torch.int8 or exps.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] < 1
+            or exps.shape != (codes.shape[0], (codes.shape[1] + GROUP - 1) // GROUP) or exps.device != codes.device):
+        raise ValueError(f"{what} expects int8 codes [rows, C] and uint8 exps [rows, ceil(C / 32)] on one device")
+
+
 def empty_codes(rows, C, device):
     """Room for the 8-bit form of [rows, C]."""
     return (torch.empty((rows, C), dtype=torch.int8, device=device),
@@ -62,7 +69,11 @@ def empty_codes(rows, C, device):
 
 
 def pack_codes(x):
-    """(codes, exps) of contiguous rows [rows, C] (``pack_rows`` without its checks)."""
+    """(codes, exps) of the rows [rows, C] (``pack_rows`` without the object around them)."""
+    _check_rows(x, "pack_rows")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"pack_rows expects [rows, C] with at least one column, got {tuple(x.shape)}")
+    x = x.detach().contiguous()
     rows, C = x.shape
     dev = x.device
     codes, exps = empty_codes(rows, C, dev)
@@ -75,10 +86,7 @@ def pack_codes(x):
 def pack_rows(x):
     """8-bit form of the rows [rows, C] of a float32, bfloat16 or float16 tensor on
     the HIP device."""
-    _check_rows(x, "pack_rows")
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise ValueError(f"pack_rows expects [rows, C] with at least one column, got {tuple(x.shape)}")
-    return PackedRows(*pack_codes(x.detach().contiguous()), x.dtype)
+    return PackedRows(*pack_codes(x), x.dtype)
 
 
 def unpack_rows(codes, exps, dtype=torch.float32):
@@ -87,9 +95,7 @@ def unpack_rows(codes, exps, dtype=torch.float32):
         raise RuntimeError("mvfusion unpack_rows runs on a HIP device only (there is no CPU fallback).")
     if dtype not in ROW_TYPES:
         raise TypeError(f"mvfusion unpack_rows gives float32, bfloat16 or float16 rows, not {dtype}")
-    if (codes.dtype != torch.int8 or exps.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] < 1
-            or exps.shape != (codes.shape[0], (codes.shape[1] + GROUP - 1) // GROUP) or exps.device != codes.device):
-        raise ValueError("unpack_rows expects int8 codes [rows, C] and uint8 exps [rows, ceil(C / 32)] on one device")
+    check_codes(codes, exps, "unpack_rows")
     codes, exps = codes.contiguous(), exps.contiguous()
     rows, C = codes.shape
     dev = codes.device

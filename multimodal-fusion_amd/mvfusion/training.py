@@ -302,7 +302,7 @@ class _BatchNormActLinear8(torch.autograd.Function):
             gy = _product(grad_out, weight.t(), None)[0]
             gz, gw, gb = _bn8_backward(gy, codes, exps, w, b, invstd, ctx.batch_stats, ctx.slope, need)
         if need[3]:
-            glw, glb = xty8(grad_out, codes, exps, tail=(w, b, ctx.slope), want_sums=need[4])
+            glw, glb = _xty8(grad_out, codes, exps, tail=(w, b, ctx.slope), want_sums=need[4])
         elif need[4]:
             glb = xty(grad_out).view(-1)
         return (gz, gw, gb, glw, glb) + (None,) * 9
@@ -480,9 +480,28 @@ class _Linear(torch.autograd.Function):
 
 
 def xty8(x, codes, exps, tail=None, want_sums=False):
-    """(x^T . y, column sums of x or None) for float32 rows x and y read from 8-bit rows
-    (mvf_xty8).  tail = (weight, bias, slope): the rows are those of
-    ``mvf_batch_norm_act8_forward`` and y the activated values made of them."""
+    """(x^T . y, column sums of x or None) for float32 rows x [rows, A] and y read from 8-bit
+    rows: codes int8 [rows, B], exps uint8 [rows, ceil(B / 32)] (mvf_xty8).  tail = (weight,
+    bias, slope): the rows are those of ``mvf_batch_norm_act8_forward`` and y the activated
+    values made of them; weight and bias float32 [B] or None, slope None: no activation."""
+    if x.dtype != torch.float32:
+        raise TypeError(f"mvfusion xty8 expects float32 rows, got {x.dtype}")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"xty8 expects rows [rows, A] with at least one column, got {tuple(x.shape)}")
+    packed.check_codes(codes, exps, "xty8")
+    if codes.shape[0] != x.shape[0] or codes.device != x.device:
+        raise ValueError(f"xty8: {codes.shape[0]} packed rows on {codes.device} do not fit {x.shape[0]} rows on {x.device}")
+    w, b, slope = tail if tail is not None else (None, None, None)
+    for t in (w, b):
+        if t is not None and (t.dtype != torch.float32 or t.shape != codes.shape[1:] or t.device != x.device):
+            raise ValueError(f"xty8: weight and bias must be float32 [{codes.shape[1]}] on the device of the rows")
+    if not x.is_cuda:
+        raise RuntimeError("mvfusion xty8 runs on a HIP device only (there is no CPU fallback).")
+    return _xty8(x, codes.contiguous(), exps.contiguous(), None if tail is None else (_vector(w), _vector(b), slope), want_sums)
+
+
+def _xty8(x, codes, exps, tail=None, want_sums=False):
+    """xty8 without its checks, for the rows a forward has kept."""
     lib = L.load()
     x = x.contiguous()
     dev = x.device
@@ -530,7 +549,7 @@ class _Linear8(torch.autograd.Function):
         gx = _product(grad_y, weight.t(), None)[0] if need[0] else None
         gw = gb = None
         if need[1]:
-            gw, gb = xty8(grad_y, codes, exps, want_sums=need[2])
+            gw, gb = _xty8(grad_y, codes, exps, want_sums=need[2])
         elif need[2]:
             gb = xty(grad_y).view(-1)
         return gx, gw, gb, None

@@ -208,3 +208,31 @@ def test_sets_that_do_not_fit(keep):
                 tr.mlp_on_rows_and_sets(seq, *bad, ptr)
         with pytest.raises(RuntimeError):
             tr.mlp_on_rows_and_sets(seq.cpu(), x, sets, ptr)
+
+
+# ---- the reduction over packed rows by itself -----------------------------------------------------------
+@pytest.mark.parametrize("tail", [False, True])
+def test_xty8_layouts(tail):
+    """Rows, codes and parameters that are not contiguous give what contiguous ones do; no rows give zeros."""
+    from mvfusion import packed, training as tr
+    torch.manual_seed(6)
+    x, y = torch.randn(1000, 24, device="cuda"), torch.randn(1000, 50, device="cuda")
+    w, b = torch.randn(2, 50, device="cuda")
+    p = packed.pack_rows(y)
+    args = (w, b, 0.2) if tail else None
+    want, sums = tr.xty8(x, p.codes, p.exps, args, want_sums=True)
+    v = p.unpack().double()
+    if tail:
+        v = v * w.double() + b.double()
+        v = torch.where(v > 0, v, v * float(np.float32(0.2)))
+    g = x.double()
+    mag = (g.abs().t().contiguous() @ (p.unpack().double().abs() * (w.double().abs() if tail else 1)
+                                       + (b.double().abs() if tail else 0))).cpu().numpy()
+    within(want.cpu().numpy(), (g.t().contiguous() @ v).cpu().numpy(), 512 * U * mag)
+    within(sums.cpu().numpy(), g.sum(0).cpu().numpy(), 64 * U * g.abs().sum(0).cpu().numpy())
+    spread = lambda t: torch.stack([t, t], -1)[..., 0]  # noqa: E731
+    got, again = tr.xty8(spread(x), spread(p.codes), spread(p.exps), (spread(w), spread(b), 0.2) if tail else None,
+                         want_sums=True)
+    assert torch.equal(got, want) and torch.equal(again, sums)
+    none, sums = tr.xty8(x[:0], p.codes[:0], p.exps[:0], args, want_sums=True)
+    assert none.shape == (24, 50) and not none.any() and not sums.any()

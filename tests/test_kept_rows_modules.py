@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.nn.utils import parametrize, prune
 
-from mvfusion import residual, training
+from mvfusion import packed, residual, training
 
 
 @pytest.mark.parametrize("keep", [None, "float32", "int8"])
@@ -73,3 +73,29 @@ def test_kernels_are_chosen_by_width_type_and_device():
     assert training._bn_plan(host, bn, bn.weight, bn.bias) is not None
     bn.running_mean = torch.zeros(16)
     assert training._bn_plan(host, bn, bn.weight, bn.bias) is None
+
+
+def test_what_xty8_and_pack_codes_refuse():
+    """The reduction over packed rows reads only what is there: rows, types and devices have to agree."""
+    x, w = torch.zeros(6, 5), torch.ones(40)
+    codes, exps = torch.zeros(6, 40, dtype=torch.int8), torch.zeros(6, 2, dtype=torch.uint8)
+    for error, args in [
+            (TypeError, (x.double(), codes, exps)), (ValueError, (x[0], codes, exps)), (ValueError, (x[:, :0], codes, exps)),
+            (ValueError, (x, codes[:5], exps[:5])), (ValueError, (x, codes, exps[:, :1])), (ValueError, (x, codes, exps[:5])),
+            (ValueError, (x, codes.float(), exps)), (ValueError, (x, codes, exps.int())), (ValueError, (x, codes[0], exps[0])),
+            (ValueError, (x, Codes(6, 40), exps)), (ValueError, (x, codes, exps, (w[:39], None, 0.2))),
+            (ValueError, (x, codes, exps, (w, w.double(), 0.2))), (ValueError, (x, codes, exps, (None, Rows(40), None))),
+            (RuntimeError, (x, codes, exps)), (RuntimeError, (x, codes, exps, (w, None, 0.2)))]:
+        with pytest.raises(error):
+            training.xty8(*args)
+    with pytest.raises(RuntimeError):
+        packed.pack_codes(x)
+    with pytest.raises(TypeError):
+        packed.pack_codes(Rows(6, 5, dtype=torch.float64))
+    with pytest.raises(ValueError):
+        packed.pack_codes(Rows(5))
+
+
+class Codes(Rows):
+    def __init__(self, *shape):
+        super().__init__(*shape, dtype=torch.int8)
