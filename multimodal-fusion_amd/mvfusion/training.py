@@ -313,11 +313,23 @@ def _takes_bn(z, bn):
             and isinstance(bn, torch.nn.BatchNorm1d) and z.shape[1] == bn.num_features)
 
 
-def _bn_plan(z, bn, weight, bias, kernel_counts=False):
-    """(running mean, running variance, batch_stats, factor, counter) of the next call on z of an
-    nn.BatchNorm1d with these parameters; None where this package's kernels do not take one of its
-    tensors.  The batch is counted in num_batches_tracked here, or, with kernel_counts, by the kernel
-    that is given the counter (None: already counted, or nothing to count)."""
+def _sums_for(z, col_sums):
+    """col_sums, refused unless they are partial sums of z's columns."""
+    if col_sums is not None and not (
+            col_sums.dtype == torch.float64 and col_sums.dim() == 3 and col_sums.shape[0] > 0
+            and col_sums.shape[1] == 2 and col_sums.shape[2] == z.shape[1] and col_sums.device == z.device
+            and col_sums.is_contiguous()):
+        raise ValueError(f"col_sums must be contiguous float64 [n, 2, {z.shape[1]}] on the device of the rows, as "
+                         f"linear(..., want_sums=True) returns them, got {tuple(col_sums.shape)} {col_sums.dtype}")
+    return col_sums
+
+
+def _bn_plan(z, bn, weight, bias, kernel_counts=False, col_sums=None):
+    """(running mean, running variance, batch_stats, factor, counter, the column sums to use) of the
+    next call on z of an nn.BatchNorm1d with these parameters; None where this package's kernels do
+    not take one of its tensors.  The batch is counted in num_batches_tracked here, or, with
+    kernel_counts, by the kernel that is given the counter (None: already counted, or nothing to
+    count)."""
     rm, rv, tracked = bn.running_mean, bn.running_var, bn.num_batches_tracked
     for t in (weight, bias, rm, rv):
         if t is not None and not (t.device == z.device and t.dtype == torch.float32 and t.shape == z.shape[1:]):
@@ -328,6 +340,7 @@ def _bn_plan(z, bn, weight, bias, kernel_counts=False):
         if z.shape[0] < 2:
             raise ValueError(
                 f"Expected more than 1 value per channel when training, got input size {tuple(z.shape)}")
+        col_sums = _sums_for(z, col_sums)
         if bn.training and bn.track_running_stats and tracked is not None:
             if kernel_counts and bn.momentum is not None and tracked.device == z.device and tracked.dtype == torch.int64:
                 counter = tracked
@@ -337,7 +350,8 @@ def _bn_plan(z, bn, weight, bias, kernel_counts=False):
     # running statistics: updated in train mode, read in eval mode, unused by an eval-mode
     # module that tracks none (it normalises with batch statistics)
     use_running = rm is not None and (bn.training or not batch_stats)
-    return (rm if use_running else None, rv if use_running else None, batch_stats, factor, counter)
+    return (rm if use_running else None, rv if use_running else None, batch_stats, factor, counter,
+            col_sums if batch_stats else None)
 
 
 def batch_norm_act(z, bn, act, col_sums=None, keep=None):
@@ -356,12 +370,11 @@ def batch_norm_act(z, bn, act, col_sums=None, keep=None):
         return act(bn(z))
     weight, bias = bn.weight, bn.bias
     keeps8 = _keeps8(keep, z, weight, bias)
-    plan = _bn_plan(z, bn, weight, bias, keeps8)
+    plan = _bn_plan(z, bn, weight, bias, keeps8, col_sums)
     if plan is None:
         return act(bn(z))
-    rm, rv, batch_stats, factor, counter = plan
+    rm, rv, batch_stats, factor, counter, col_sums = plan
     slope = float(act.negative_slope) if fused_act else None
-    col_sums = col_sums if batch_stats else None
     if keeps8:
         y = _BatchNormAct8.apply(z, weight, bias, rm, rv, bn.eps, slope, batch_stats, factor, counter, col_sums)
     else:
@@ -376,12 +389,12 @@ def batch_norm_act_linear(z, bn, act, lin, col_sums=None, want_sums=False, keep=
     if isinstance(act, torch.nn.LeakyReLU) and _takes(lin, z) and _takes_bn(z, bn):
         weight, bias = bn.weight, bn.bias
         if _keeps8(keep, z, weight, bias, lin.weight, lin.bias):
-            plan = _bn_plan(z, bn, weight, bias, True)
+            plan = _bn_plan(z, bn, weight, bias, True, col_sums)
             if plan is not None:
-                rm, rv, batch_stats, factor, counter = plan
+                rm, rv, batch_stats, factor, counter, col_sums = plan
                 y, sums = _BatchNormActLinear8.apply(
                     z, weight, bias, lin.weight, lin.bias, rm, rv, bn.eps, float(act.negative_slope),
-                    batch_stats, factor, counter, col_sums if batch_stats else None, bool(want_sums))
+                    batch_stats, factor, counter, col_sums, bool(want_sums))
                 return (y, sums) if want_sums else y
     form = {} if keep is None else {"keep": keep}
     return linear(lin, batch_norm_act(z, bn, act, col_sums=col_sums, **form), want_sums, **form)

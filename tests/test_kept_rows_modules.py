@@ -99,3 +99,13 @@ def test_what_xty8_and_pack_codes_refuse():
 class Codes(Rows):
     def __init__(self, *shape):
         super().__init__(*shape, dtype=torch.int8)
+
+
+def test_column_sums_that_do_not_fit():
+    """The statistics' kernel reads n rows of 2 C float64 sums."""
+    z, sums = torch.zeros(6, 8), torch.zeros(4, 2, 8, dtype=torch.float64)
+    assert training._sums_for(z, sums) is sums and training._sums_for(z, None) is None
+    for bad in (sums.float(), sums[:, :, :4], sums[:, :1], sums[:0], sums[0], torch.zeros(4, 2, 9, dtype=torch.float64),
+                sums.transpose(0, 1).contiguous().transpose(0, 1)):
+        with pytest.raises(ValueError):
+            training._sums_for(z, bad)
