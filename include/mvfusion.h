@@ -517,7 +517,9 @@ int mvf_unpack_rows8(
  * forward: y [rows][C] (bit for bit the value of mvf_batch_norm_act_forward; may
  * be NULL), codes / exps of zhat (computed in float64), save_invstd [C].  With an
  * activation a code reads back on the side of the kink -beta / gamma (rounded
- * to float32) on which the value lies: it is moved by at most one step for that.
+ * to float32) on which the value lies: it is moved by at most one step for that,
+ * and a group in which a value of at least 127 steps meets a kink of 127 to 128
+ * steps is kept in the next step (e + 1), where there is a code past the kink.
  * num_batches (may be NULL): a counter that training adds 1 to.
  * backward: the formulas of mvf_batch_norm_act_backward with zhat as read back
  * and the activation's side taken from it; grad_z, grad_weight, grad_bias may be

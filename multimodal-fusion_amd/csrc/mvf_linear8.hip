@@ -94,9 +94,9 @@ __global__ __launch_bounds__(L8_FWD_THREADS) void linear8_forward_kernel(
     __shared__ __attribute__((aligned(16))) char wlds[32 * NO * PITCH_I];
     __shared__ __attribute__((aligned(16))) float blds[32 * NO];
     // BatchNorm's terms of the columns: float64 mean and 1 / spread; the same in float32, weight, bias;
-    // the kink's sign and place
+    // the kink's sign, place and last value
     __shared__ __attribute__((aligned(16))) double tlds[TAIL ? 2 * I : 1];
-    __shared__ __attribute__((aligned(16))) float flds[TAIL ? 6 * I : 1];
+    __shared__ __attribute__((aligned(16))) float flds[TAIL ? 7 * I : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, kh = lane >> 5;
     const int oq = O >> 2;
@@ -121,6 +121,7 @@ __global__ __launch_bounds__(L8_FWD_THREADS) void linear8_forward_kernel(
             flds[3 * I + c] = beta;
             flds[4 * I + c] = k.sign;
             flds[5 * I + c] = k.at;
+            flds[6 * I + c] = __uint_as_float(bn.act ? k.last() : 0x7f800000u);
         }
     }
     __syncthreads();
@@ -156,12 +157,12 @@ __global__ __launch_bounds__(L8_FWD_THREADS) void linear8_forward_kernel(
         constexpr bool WHOLE = decltype(how)::WHOLE;
         unsigned *qdst = (unsigned *)(codes + (size_t)t * L8_ROWS * I);
         uint8_t *edst = exps + (size_t)t * L8_ROWS * GR;
-        float terms[6][4];          // mean, 1 / spread, gamma, beta, kink
+        float terms[7][4];          // mean, 1 / spread, gamma, beta, kink
         double terms64[2][4];
         if constexpr (TAIL) {
             const int c = (int)l8_fresh((unsigned)col);
 #pragma unroll
-            for (int i = 0; i < 6; ++i) {
+            for (int i = 0; i < 7; ++i) {
                 const l8_f4 v = *(const l8_f4 *)(flds + i * I + c);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) terms[i][k] = v[k];
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(L8_FWD_THREADS) void linear8_forward_kernel(
                 for (int k = 0; k < 4; ++k) {
                     zh[k] = ((double)v[k] - terms64[0][k]) * terms64[1][k];
                     zf[k] = (float)zh[k];
-                    m = max(m, r8_magnitude(zf[k]));
+                    m = BnKink::most(m, zf[k], __float_as_uint(terms[6][k]));
                 }
                 e = r8_exponent(l8_group_max<IQ>(m), R8_E_MAX);
 #pragma unroll

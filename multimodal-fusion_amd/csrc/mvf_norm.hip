@@ -462,8 +462,8 @@ static BnQuarters bn_quarters(const BnGrid &g, int rpp)
 template <bool VEC>
 __device__ __forceinline__ void bn_apply8_row(
     const float (&v)[4], i64 r, int col, int C, int G, bool live, const double (&mean64)[4], const double (&invstd64)[4],
-    const float (&gamma)[4], const float (&beta)[4], const BnKink (&kink)[4], int act, float slope,
-    float *y, int8_t *codes, uint8_t *exps)
+    const float (&gamma)[4], const float (&beta)[4], const BnKink (&kink)[4], const unsigned (&last)[4],
+    int act, float slope, float *y, int8_t *codes, uint8_t *exps)
 {
     double zh[4];
     unsigned m = 0;
@@ -472,7 +472,7 @@ __device__ __forceinline__ void bn_apply8_row(
     for (int j = 0; j < 4; ++j) {
         zh[j] = ((double)v[j] - mean64[j]) * invstd64[j];
         zf[j] = (float)zh[j];
-        if (VEC ? live : col + j < C) m = max(m, r8_magnitude(zf[j]));
+        if (VEC ? live : col + j < C) m = BnKink::most(m, zf[j], last[j]);
     }
     const int e = r8_exponent(r8_max8(m), R8_E_MAX);
     int q[4];
@@ -507,6 +507,7 @@ __global__ __launch_bounds__(BN_THREADS) void bn_apply8_kernel(
     float gamma[4], beta[4];
     double mean64[4], invstd64[4];
     BnKink kink[4];
+    unsigned last[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int c = min(w.col + j, C - 1);
@@ -515,9 +516,10 @@ __global__ __launch_bounds__(BN_THREADS) void bn_apply8_kernel(
         gamma[j] = weight ? weight[c] : 1.0f;
         beta[j] = bias ? bias[c] : 0.0f;
         kink[j].load(gamma[j], beta[j]);
+        last[j] = act ? kink[j].last() : 0x7f800000u;
     }
     auto one = [&](i64 r, const float (&v)[4]) {
-        bn_apply8_row<VEC>(v, r, w.col, C, G, live, mean64, invstd64, gamma, beta, kink, act, slope, y, codes, exps);
+        bn_apply8_row<VEC>(v, r, w.col, C, G, live, mean64, invstd64, gamma, beta, kink, last, act, slope, y, codes, exps);
     };
     i64 r = w.r0;
     for (; r + 3 * (i64)w.rstep < w.rend; r += 4 * (i64)w.rstep) {
@@ -634,6 +636,7 @@ __global__ __launch_bounds__(BN_SMALL_THREADS) void bn_small8_forward_kernel(
     float gamma[4], beta[4];
     double mean64[4], invstd64[4];
     BnKink kink[4];
+    unsigned last[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int c = min(col + j, C - 1);
@@ -642,6 +645,7 @@ __global__ __launch_bounds__(BN_SMALL_THREADS) void bn_small8_forward_kernel(
         gamma[j] = weight ? weight[c] : 1.0f;
         beta[j] = bias ? bias[c] : 0.0f;
         kink[j].load(gamma[j], beta[j]);
+        last[j] = act ? kink[j].last() : 0x7f800000u;
     }
     for (int r = r0; r < rows; r += 2 * BN_SMALL_LANES) {
         float v[2][4];
@@ -651,7 +655,7 @@ __global__ __launch_bounds__(BN_SMALL_THREADS) void bn_small8_forward_kernel(
         for (int u = 0; u < 2; ++u) {
             const int ru = r + u * BN_SMALL_LANES;
             if (ru >= rows) break;
-            bn_apply8_row<VEC>(v[u], ru, col, C, G, live, mean64, invstd64, gamma, beta, kink, act, slope, y, codes, exps);
+            bn_apply8_row<VEC>(v[u], ru, col, C, G, live, mean64, invstd64, gamma, beta, kink, last, act, slope, y, codes, exps);
         }
     }
 }

@@ -236,3 +236,90 @@ def test_xty8_layouts(tail):
     assert torch.equal(got, want) and torch.equal(again, sums)
     none, sums = tr.xty8(x[:0], p.codes[:0], p.exps[:0], args, want_sums=True)
     assert none.shape == (24, 50) and not none.any() and not sums.any()
+
+
+# ---- kinks at the end of the codes' range --------------------------------------------------------------
+def sided_codes(zh, gamma, beta):
+    """(codes, exps) of normalised rows: the code nearest to the value on its own side of the kink; a group in
+    which a value of at least 127 steps meets a kink of 127 to 128 steps takes the next step."""
+    C = zh.shape[1]
+    t = (-beta.astype(np.float32) / gamma.astype(np.float32)).astype(np.float64)
+    on, up = zh * gamma + beta > 0, gamma > 0
+    zf = zh.astype(np.float32)
+    e = ref.exponents(zf)
+    at = np.ldexp(np.broadcast_to(t, zh.shape), ref.BIAS - ref.spread(e, C))
+    past = np.zeros((zh.shape[0], e.shape[1] * ref.GROUP), bool)
+    past[:, :C] = (np.abs(zf) >= np.ldexp(127.0, ref.spread(e, C) - ref.BIAS)) & (np.floor(np.abs(at)) == 127)
+    e = e + past.reshape(*e.shape, ref.GROUP).any(2)
+    q = np.clip(ref.codes_of(zh, e), -127, 127)
+    at = np.ldexp(np.broadcast_to(t, zh.shape), ref.BIAS - ref.spread(e, C))
+    q = np.where(on, np.where(up, np.fmax(q, np.floor(at) + 1), np.fmin(q, np.ceil(at) - 1)),
+                 np.where(up, np.fmin(q, np.floor(at)), np.fmax(q, np.ceil(at))))
+    assert np.abs(q).max() <= 127
+    return q.astype(np.int8), e.astype(np.uint8)
+
+
+def rows_at_the_end(rows, C, g):
+    """(z, gamma, beta): kinks of either sign between 127 and 127.5 steps of 1/64, some at the ends of that range
+    and some elsewhere, and rows whose largest values lie on both sides of them."""
+    gamma = np.where(g.random(C) < 0.5, -1.0, 1.0) * 2.0 ** g.integers(-1, 2, C)
+    kink = (127 + g.choice([0.0, 0.03, 0.2, 0.4, 0.49, 0.5], C)) / 64 * np.where(g.random(C) < 0.5, -1, 1)
+    kink[::3] = g.normal(size=len(kink[::3]))
+    beta = (-kink * gamma).astype(np.float32)
+    z = g.uniform(-1.9, 1.9, (rows, C))
+    near = g.random((rows, C)) < 0.1
+    z = np.where(near, np.sign(kink) * (127 + g.uniform(-0.6, 0.5, (rows, C))) / 64, z)
+    z = np.where(g.random((rows, C)) < 0.02, kink, z)
+    z *= 2.0 ** np.where(g.random((rows, 1)) < 0.1, -1, 0)
+    return z.astype(np.float32), gamma.astype(np.float32), beta
+
+
+@pytest.mark.parametrize("rows,C,O", [(40, 33, 0), (900, 64, 0), (3000, 50, 0), (2500, 32, 0), (5000, 6, 0), (3001, 8, 8),
+                                      (3001, 16, 40), (3001, 32, 16), (3001, 64, 64), (3001, 33, 9)])
+def test_kept_side_at_the_end_of_the_range(rows, C, O):
+    """Eval mode with statistics that make the normalised value z itself.  Bounds: the product, the slope and the
+    scale are three float32 operations behind g, or behind g W with O + 2."""
+    from mvfusion import training as tr
+    g = np.random.default_rng(rows + C)
+    z, gamma, beta = rows_at_the_end(rows, C, g)
+    bn = torch.nn.BatchNorm1d(C, eps=0.0).cuda().eval()
+    with torch.no_grad():
+        bn.weight.copy_(T(gamma))
+        bn.bias.copy_(T(beta))
+    codes, exps = sided_codes(z.astype(np.float64), gamma.astype(np.float64), beta.astype(np.float64))
+    plain = ref.exponents(z)
+    assert 0 < (exps > plain).sum() < 0.8 * exps.size
+    x, act = T(z).cuda().requires_grad_(True), torch.nn.LeakyReLU(0.125)
+    if O:
+        lin = torch.nn.Linear(C, O).cuda()
+        y = tr.batch_norm_act_linear(x, bn, act, lin, keep="int8")
+        w64 = lin.weight.detach().cpu().double().numpy()
+    else:
+        y, w64 = tr.batch_norm_act(x, bn, act, keep="int8"), np.eye(C)
+    got = [t.cpu().numpy() for t in y.grad_fn.saved_tensors[:2]]
+    assert np.array_equal(got[0], codes) and np.array_equal(got[1], exps)
+    zq, on = ref.unpack(codes, exps), z.astype(np.float64) * gamma + beta > 0
+    assert np.array_equal(ref.bn_on(zq, gamma.astype(np.float64), beta.astype(np.float64)), on)
+    assert np.all(np.abs(zq - z) <= np.ldexp(1.0, ref.spread(exps.astype(np.int64), C) - ref.BIAS))
+    gy = g.normal(size=(rows, O or C)).astype(np.float32)
+    gx, dgamma, dbeta = (t.cpu().numpy() for t in torch.autograd.grad(y, (x, bn.weight, bn.bias), T(gy).cuda()))
+    t = np.where(on, 1.0, 0.125)
+    gh, mag = t * (gy.astype(np.float64) @ w64), np.abs(gy.astype(np.float64)) @ np.abs(w64)
+    within(gx, gh * gamma, (O + 5) * U * mag * np.abs(gamma), "z")
+    within(dbeta, gh.sum(0), 1024 * U * mag.sum(0), "beta")
+    within(dgamma, (gh * zq).sum(0), 1024 * U * (mag * np.abs(zq)).sum(0), "gamma")
+
+
+def test_idle_columns_take_no_part_in_a_group():
+    """Lanes past the last column hold no value: they must not send their group to the next step."""
+    from mvfusion import training as tr
+    for rows in (300, 2000):
+        z = np.full((rows, 5), 0.5, np.float32)
+        bn = torch.nn.BatchNorm1d(5, eps=0.0).cuda().eval()
+        with torch.no_grad():
+            bn.running_mean[4], bn.running_var[4] = -1e4, 1.0       # (an idle column would read as 1e4)
+            bn.bias[4] = -50.0
+        z[:, 4] = -1e4
+        y = tr.batch_norm_act(T(z).cuda().requires_grad_(True), bn, torch.nn.LeakyReLU(0.2), keep="int8")
+        codes, exps = (t.cpu().numpy() for t in y.grad_fn.saved_tensors[:2])
+        assert (codes[:, :4] == 64).all() and not codes[:, 4].any() and (exps == 126).all()
