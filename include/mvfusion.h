@@ -544,7 +544,7 @@ int mvf_batch_norm_act8_backward(
  * and 0; act, slope as there), i.e. the Linear behind that activation.
  * x_sums (may be NULL): [A] the column sums of x, the bias gradient.  codes and
  * exps are contiguous rows of B columns.  bf16 matrix cores, float32 operands cut
- * exactly into bf16 parts, float32 accumulators, partial sums folded in a fixed
+ * exactly into bf16 parts, float32 sums to the nearest, partial sums folded in a fixed
  * order (the same bits on every run).  workspace: mvf_xty8_workspace_bytes(). */
 size_t mvf_xty8_workspace_bytes(void);
 int mvf_xty8(

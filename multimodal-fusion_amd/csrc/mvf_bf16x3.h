@@ -15,6 +15,11 @@ __device__ __forceinline__ xty_acc xty_mfma16(xty_u4 a, xty_u4 b, xty_acc c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(xty_bf8, a), __builtin_bit_cast(xty_bf8, b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ xty_acc xty_zero()
+{
+    return xty_acc{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+}
+
 // high halves of two floats as two bf16 (the first in the low half)
 __device__ __forceinline__ unsigned xty_hi2(float a, float b)
 {
@@ -41,11 +46,29 @@ template <int PARTS> struct XtyParts {
     }
 };
 
+// 16 rows' part of the sums, the smallest parts first
+__device__ __forceinline__ xty_acc xty_product(const XtyParts<3> &x, xty_u4 y)
+{
+    return xty_mfma16(x.p[0], y, xty_mfma16(x.p[1], y, xty_mfma16(x.p[2], y, xty_zero())));
+}
+
+// Behind every addition of a product: the sums are formed here.  The product's registers are free for the next
+// one, and no branch comes between the two (hipcc counts the waits that a matrix instruction's result needs along
+// one side of a branch only: without this, rows of 32 -> 32 columns without bias gave wrong sums).
+__device__ __forceinline__ void xty_done(xty_acc &sum)
+{
+    asm volatile("" : "+v"(sum));
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // The matrix cores add bf16 products to float32 sums by cutting off what does not fit, towards minus
-// infinity: over 2 M rows that shifts sums of zero-mean terms by 2e-6 of their typical size.  Odd
-// waves therefore sum the negated products (one operand's sign turned, by a factor or in its two
-// bf16) and are subtracted where waves are joined: the two halves' errors cancel.  (Sums of terms of one
-// sign, which the same rounding makes shorter in every wave, end up to 6e-7 of themselves short at 2 M rows.)
+// infinity.  Sums of one sign kept in one accumulator over all rows come out 4e-6 of themselves short at 8 M
+// rows, and more than in proportion beyond; sums of zero-mean terms are moved together, by 2e-6 of their
+// typical size at 2 M.  So every 16 rows are a product of their own, from zero, which the vector unit adds to the
+// wave's float32 sums, to the nearest (Linear of 2 M x 64 -> 64, forward and backward, 505 -> 510 us; error of
+// zero-mean sums 3e-7 -> 1.6e-7, of one sign that of their last rounding).  What a product still cuts off
+// downwards cancels between the waves: odd ones sum the negated products (one operand's sign turned, by a factor
+// or in its two bf16) and are subtracted where waves are joined, in float64 from the workgroup on.
 __device__ __forceinline__ float xty_turned(int wave) { return wave & 1 ? -1.0f : 1.0f; }
 __device__ __forceinline__ unsigned xty_flip(int wave) { return wave & 1 ? 0x80008000u : 0u; }
 

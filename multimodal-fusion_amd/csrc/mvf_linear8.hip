@@ -466,9 +466,10 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
                     for (int k = 0; k < 4; ++k)
                         yp[k] = __builtin_amdgcn_perm(d[2 * k + 1], d[2 * k], b == 0 ? 0x05040100u : 0x07060302u) ^ flip;
 #pragma unroll
-                    for (int p = 2; p >= 0; --p)
-#pragma unroll
-                        for (int i = 0; i < NA; ++i) run[i][b] = xty_mfma16(gp[i].p[p], yp, run[i][b]);
+                    for (int i = 0; i < NA; ++i) {
+                        run[i][b] += xty_product(gp[i], yp);
+                        xty_done(run[i][b]);
+                    }
                 }
             }
         }
@@ -726,12 +727,15 @@ __global__ __launch_bounds__(T8_THREADS) void tail8_sums_kernel(
                     ap[k] = zp[k] & up;
                     op[k] = 0x3f803f80u & up;               // (1.0 twice)
                 }
-#pragma unroll
-                for (int p = 2; p >= 0; --p) {
-                    all[b] = xty_mfma16(gp.p[p], zp, all[b]);
-                    above[b] = xty_mfma16(gp.p[p], ap, above[b]);
-                    on[b] = xty_mfma16(gp.p[p], op, on[b]);
-                }
+                // (two products under way at a time: the registers hold no third)
+                const xty_acc a = xty_product(gp, zp), m = xty_product(gp, ap);
+                all[b] += a;
+                xty_done(all[b]);
+                const xty_acc o = xty_product(gp, op);
+                above[b] += m;
+                xty_done(above[b]);
+                on[b] += o;
+                xty_done(on[b]);
             }
         }
         l8_wave_sync();

@@ -258,7 +258,7 @@ __global__ __launch_bounds__(XTY_FOLD_SLOTS * XTY_FOLD_SLICES) void xty_fold_ker
 // bf16 matrix cores (v_mfma_f32_32x32x16_bf16, 16 times the rate of the float32 form).  A value read
 // back has 7 significant bits and a power of two: one bf16 holds it exactly.  A float32 x is cut
 // into three bf16 parts by truncation (8 + 8 + 8 bits, exact), so RAW is three products per block,
-// each exact, accumulated in float32; TAIL cuts y into three parts as well and takes the six
+// each exact, added up in float32; TAIL cuts y into three parts as well and takes the six
 // products above 2^-24 of the result.  (A magnitude that is not finite in x, or NaN in y, makes
 // the sums it enters NaN.)
 //
@@ -394,17 +394,16 @@ __global__ __launch_bounds__(XTY_THREADS) void xty8_kernel(
 #pragma unroll
             for (int i = 0; i < NA; ++i) {
                 if constexpr (TAIL) {
-                    acc[i][j] = xty_mfma16(xp[i].p[2], yp.p[0], acc[i][j]);
-                    acc[i][j] = xty_mfma16(xp[i].p[1], yp.p[1], acc[i][j]);
-                    acc[i][j] = xty_mfma16(xp[i].p[0], yp.p[2], acc[i][j]);
-                    acc[i][j] = xty_mfma16(xp[i].p[1], yp.p[0], acc[i][j]);
-                    acc[i][j] = xty_mfma16(xp[i].p[0], yp.p[1], acc[i][j]);
-                    acc[i][j] = xty_mfma16(xp[i].p[0], yp.p[0], acc[i][j]);
+                    xty_acc part = xty_mfma16(xp[i].p[2], yp.p[0], xty_zero());
+                    part = xty_mfma16(xp[i].p[1], yp.p[1], part);
+                    part = xty_mfma16(xp[i].p[0], yp.p[2], part);
+                    part = xty_mfma16(xp[i].p[1], yp.p[0], part);
+                    part = xty_mfma16(xp[i].p[0], yp.p[1], part);
+                    acc[i][j] += xty_mfma16(xp[i].p[0], yp.p[0], part);
                 } else {
-                    acc[i][j] = xty_mfma16(xp[i].p[2], yp.p[0], acc[i][j]);
-                    acc[i][j] = xty_mfma16(xp[i].p[1], yp.p[0], acc[i][j]);
-                    acc[i][j] = xty_mfma16(xp[i].p[0], yp.p[0], acc[i][j]);
+                    acc[i][j] += xty_product(xp[i], yp.p[0]);
                 }
+                xty_done(acc[i][j]);
             }
         }
     };

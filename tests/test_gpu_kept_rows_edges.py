@@ -323,3 +323,69 @@ def test_idle_columns_take_no_part_in_a_group():
         y = tr.batch_norm_act(T(z).cuda().requires_grad_(True), bn, torch.nn.LeakyReLU(0.2), keep="int8")
         codes, exps = (t.cpu().numpy() for t in y.grad_fn.saved_tensors[:2])
         assert (codes[:, :4] == 64).all() and not codes[:, 4].any() and (exps == 126).all()
+
+
+# ---- long sums -----------------------------------------------------------------------------------------
+def over_rows(g, v):
+    out = torch.zeros(g.shape[1], v.shape[1], dtype=torch.float64, device="cuda")
+    for k in range(0, g.shape[0], 1 << 18):
+        out += g[k:k + (1 << 18)].double().t().contiguous() @ v[k:k + (1 << 18)].double()
+    return out
+
+
+def long_sums(op, x, gy, lin, bn):
+    """(weight gradient and, for the block, BatchNorm's gradients, what they are in float64)."""
+    from mvfusion import packed, training as tr
+    if op == "linear":
+        y = tr.linear(lin, x, keep="int8")
+        _, gw = torch.autograd.grad(y, (x, lin.weight), gy)
+        return [gw], [over_rows(gy, packed.pack_rows(x).unpack())]
+    y = tr.batch_norm_act_linear(x, bn, torch.nn.LeakyReLU(0.25), lin, keep="int8")
+    _, gw, db = torch.autograd.grad(y, (x, lin.weight, bn.bias), gy)
+    beta = bn.bias.detach()
+    _, codes, exps, _ = tr._bn8_forward(x.detach(), bn.weight.detach(), beta, None, None, bn.eps, 0.25, True, 0.0, None, None)
+    zq = packed.unpack_rows(codes, exps)
+    t = torch.where(zq > -beta, 1.0, 0.25)
+    want, wb = torch.zeros_like(gw, dtype=torch.float64), torch.zeros_like(db, dtype=torch.float64)
+    for k in range(0, x.shape[0], 1 << 18):
+        part = slice(k, k + (1 << 18))
+        want += over_rows(gy[part], (zq[part].double() + beta.double()) * t[part])
+        wb += ((gy[part].double() @ lin.weight.detach().double()) * t[part]).sum(0)
+    return [gw, db], [want, wb]
+
+
+@pytest.mark.parametrize("op", ["linear", "block"])
+@pytest.mark.parametrize("I,O", [(64, 64), (32, 32), (64, 40), (33, 9)])
+def test_long_sums_of_one_sign(I, O, op):
+    """2^23 positive terms a sum.  Its last rounding is u; a wave adds N = 256 parts (of 16 rows) to the nearest,
+    each off by at most u of a sum that grows evenly: a deviation of u sqrt(N) / 3 of the wave's sum, and for the
+    mean of 1024 waves or more 0.17 u; what the matrix instructions cut off, always downwards, odd and even waves
+    turn opposite ways.  2 u leaves six deviations."""
+    rows = 1 << 23
+    torch.manual_seed(7)
+    x = 1 + 0.2 * torch.randn(rows, I, device="cuda").abs_()
+    gy = 0.5 + torch.rand(rows, O, device="cuda")
+    lin, bn = torch.nn.Linear(I, O, bias=False).cuda(), torch.nn.BatchNorm1d(I).cuda()
+    with torch.no_grad():
+        lin.weight.abs_()
+        bn.bias.fill_(2.5)
+    for got, want in zip(*long_sums(op, x.requires_grad_(True), gy, lin, bn)):
+        assert float(want.min()) > 0
+        assert float(((got.double() - want) / want).abs().max()) <= 2 * U
+
+
+@pytest.mark.parametrize("op", ["linear", "block"])
+@pytest.mark.parametrize("I,O", [(64, 64), (64, 40), (33, 9)])
+def test_long_sums_of_both_signs(I, O, op):
+    """2 M terms of both signs: sums grow as the root of their terms, so N additions a wave leave a deviation of
+    u sqrt(N / 6) of the result's spread: 1024 waves (two steps of 16 rows a tile) at least, N = 123 at most."""
+    rows = 2_000_000
+    torch.manual_seed(8)
+    x, gy = torch.randn(rows, I, device="cuda", requires_grad=True), torch.randn(rows, O, device="cuda")
+    lin, bn = torch.nn.Linear(I, O, bias=False).cuda(), torch.nn.BatchNorm1d(I).cuda()
+    got, want = (t[0] for t in long_sums(op, x, gy, lin, bn))
+    waves = 1024 if op == "block" and O > 32 and I % 8 == 0 else 2048
+    n = 2 * rows / 32 / waves
+    err, spread = got.double() - want, want.square().mean().sqrt()
+    assert float(err.std()) <= ((n / 6) ** 0.5 + 1) * U * float(spread)
+    assert abs(float(err.mean())) <= 0.5 * float(err.std())
