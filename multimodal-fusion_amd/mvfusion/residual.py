@@ -33,7 +33,8 @@ def _norm_args(norm, C, x, name):
     if tuple(norm.normalized_shape) != (C,):
         raise ValueError(f"residual_norm: {name} normalises {tuple(norm.normalized_shape)}, the rows have {C} channels")
     eps = torch.finfo(x.dtype).eps if norm.eps is None else float(norm.eps)
-    return kind, _vector(norm.weight, C, x, name), _vector(getattr(norm, "bias", None), C, x, name), eps
+    bias = norm.bias if kind == _LAYER else None        # (an RMS norm has none)
+    return kind, _vector(norm.weight, C, x, name), _vector(bias, C, x, name), eps
 
 
 def _vector(t, C, x, name):
