@@ -46,10 +46,10 @@ template <int PARTS> struct XtyParts {
     }
 };
 
-// 16 rows' part of the sums, the smallest parts first
-__device__ __forceinline__ xty_acc xty_product(const XtyParts<3> &x, xty_u4 y)
+// c and 16 rows' part of the sums, the smallest parts first
+__device__ __forceinline__ xty_acc xty_product(const XtyParts<3> &x, xty_u4 y, xty_acc c)
 {
-    return xty_mfma16(x.p[0], y, xty_mfma16(x.p[1], y, xty_mfma16(x.p[2], y, xty_zero())));
+    return xty_mfma16(x.p[0], y, xty_mfma16(x.p[1], y, xty_mfma16(x.p[2], y, c)));
 }
 
 // Behind every addition of a product: the sums are formed here.  The product's registers are free for the next
@@ -64,9 +64,9 @@ __device__ __forceinline__ void xty_done(xty_acc &sum)
 // The matrix cores add bf16 products to float32 sums by cutting off what does not fit, towards minus
 // infinity.  Sums of one sign kept in one accumulator over all rows come out 4e-6 of themselves short at 8 M
 // rows, and more than in proportion beyond; sums of zero-mean terms are moved together, by 2e-6 of their
-// typical size at 2 M.  So every 16 rows are a product of their own, from zero, which the vector unit adds to the
-// wave's float32 sums, to the nearest (Linear of 2 M x 64 -> 64, forward and backward, 505 -> 510 us; error of
-// zero-mean sums 3e-7 -> 1.6e-7, of one sign that of their last rounding).  What a product still cuts off
+// typical size at 2 M.  So every 16 (or 32) rows are a product of their own, from zero, which the vector unit adds
+// to the wave's float32 sums, to the nearest (Linear of 2 M x 64 -> 64, forward and backward, 505 -> 510 us; error
+// of zero-mean sums 3e-7 -> 1.6e-7, of one sign that of their last rounding).  What a product still cuts off
 // downwards cancels between the waves: odd ones sum the negated products (one operand's sign turned, by a factor
 // or in its two bf16) and are subtracted where waves are joined, in float64 from the workgroup on.
 __device__ __forceinline__ float xty_turned(int wave) { return wave & 1 ? -1.0f : 1.0f; }

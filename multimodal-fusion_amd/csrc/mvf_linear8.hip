@@ -467,7 +467,7 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
                         yp[k] = __builtin_amdgcn_perm(d[2 * k + 1], d[2 * k], b == 0 ? 0x05040100u : 0x07060302u) ^ flip;
 #pragma unroll
                     for (int i = 0; i < NA; ++i) {
-                        run[i][b] += xty_product(gp[i], yp);
+                        run[i][b] += xty_product(gp[i], yp, xty_zero());
                         xty_done(run[i][b]);
                     }
                 }
@@ -588,10 +588,12 @@ __global__ __launch_bounds__(l8_bwd_threads(KO, KI)) void linear8_backward_kerne
 //   P = g^T (t zq) = s g^T zq + (1 - s) g^T (on zq),      Q = g^T t = s sum g + (1 - s) g^T on
 // grad_W = gamma P + beta Q, and BatchNorm's column sums, of t (g W) and t (g W) zq, are the columns of
 // W . Q and W . P: neither g W nor the activated rows are formed.  zq, on zq and on are exact in one bf16, so
-// the three products are nine of the bf16 matrix cores', exact but for their float32 sums.  2 M rows of
-// 64 -> 64 columns take 203 us (with g W and the activated rows formed: 337), 161 of them without the
-// products, 128 for the bytes.  Past 32 columns of g two waves share a tile, 32 columns each: three sums of
-// 64 x 64 would leave room for one wave per SIMD (four waves a tile, of 32 x 32 sums: 227 to 253 us).
+// the three products are nine of the bf16 matrix cores', exact but for the additions; a tile of 32 rows is one
+// product from zero (mvf_bf16x3.h), added to the wave's sums by the vector unit.  2 M rows of 64 -> 64 columns
+// take 215 us in the kernel trace (added per 16 rows: 225; with the sums kept in the matrix cores' accumulators,
+// and their errors: 196 to 203, 161 of them without the products, 128 for the bytes).  Past 32 columns of g two
+// waves share a tile, 32 columns each: three sums of 64 x 64 would leave room for one wave per SIMD (four waves a
+// tile, of 32 x 32 sums, in accumulators: 227 to 253 us).
 template <int KO, int KI, bool EXACT>
 __global__ __launch_bounds__(T8_THREADS) void tail8_sums_kernel(
     const float *gsrc, int O_, const int8_t *codes, const uint8_t *exps, i64 rows, L8Bn bn, float *partial, float *partial_sums)
@@ -700,43 +702,41 @@ __global__ __launch_bounds__(T8_THREADS) void tail8_sums_kernel(
         if constexpr (decltype(how)::NEXT) load_tile(next, L8_ROWS);
         __builtin_amdgcn_sched_barrier(0);
         l8_wave_sync();
-        // lane = column, 8 rows of 16
+        // lane = column, 8 rows of 16, twice
+        XtyParts<3> gp[2];
+        unsigned d[2][8];
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
             float c[8];
-            unsigned d[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const int r = 16 * st + 8 * kh + k;
                 c[k] = *(const float *)(buf + r * PITCH_G + gc * 4);
                 const char *qt = plane + r * PITCH_Q + qc * 2;
-                d[k] = (NI == 2 ? *(const unsigned *)qt : (unsigned)*(const unsigned short *)qt) ^ signs;
+                d[st][k] = (NI == 2 ? *(const unsigned *)qt : (unsigned)*(const unsigned short *)qt) ^ signs;
             }
             sums += ((c[0] + c[1]) + (c[2] + c[3])) + ((c[4] + c[5]) + (c[6] + c[7]));
-            XtyParts<3> gp;
-            gp.cut(c);
+            gp[st].cut(c);
+        }
 #pragma unroll
-            for (int b = 0; b < NI; ++b) {
-                xty_u4 zp, ap, op;
+        for (int b = 0; b < NI; ++b) {
+            xty_u4 zp[2], up[2];
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const unsigned lo = d[2 * k], hi = d[2 * k + 1];
-                    zp[k] = __builtin_amdgcn_perm(hi, lo, b == 0 ? 0x05040100u : 0x07060302u);
-                    unsigned up = __uint_as_float(b == 0 ? lo << 16 : lo & 0xffff0000u) > at[b] ? 0xffffu : 0u;
-                    up = __uint_as_float(b == 0 ? hi << 16 : hi & 0xffff0000u) > at[b] ? up | 0xffff0000u : up;
-                    ap[k] = zp[k] & up;
-                    op[k] = 0x3f803f80u & up;               // (1.0 twice)
+                    const unsigned lo = d[st][2 * k], hi = d[st][2 * k + 1];
+                    zp[st][k] = __builtin_amdgcn_perm(hi, lo, b == 0 ? 0x05040100u : 0x07060302u);
+                    unsigned u = __uint_as_float(b == 0 ? lo << 16 : lo & 0xffff0000u) > at[b] ? 0xffffu : 0u;
+                    up[st][k] = __uint_as_float(b == 0 ? hi << 16 : hi & 0xffff0000u) > at[b] ? u | 0xffff0000u : u;
                 }
-                // (two products under way at a time: the registers hold no third)
-                const xty_acc a = xty_product(gp, zp), m = xty_product(gp, ap);
-                all[b] += a;
-                xty_done(all[b]);
-                const xty_acc o = xty_product(gp, op);
-                above[b] += m;
-                xty_done(above[b]);
-                on[b] += o;
-                xty_done(on[b]);
-            }
+            auto add = [&](xty_acc &sum, xty_u4 y0, xty_u4 y1) {
+                sum += xty_product(gp[1], y1, xty_product(gp[0], y0, xty_zero()));
+                xty_done(sum);
+            };
+            add(all[b], zp[0], zp[1]);
+            add(above[b], zp[0] & up[0], zp[1] & up[1]);
+            add(on[b], up[0] & 0x3f803f80u, up[1] & 0x3f803f80u);       // (1.0 twice)
         }
         l8_wave_sync();
     };

@@ -401,7 +401,7 @@ __global__ __launch_bounds__(XTY_THREADS) void xty8_kernel(
                     part = xty_mfma16(xp[i].p[0], yp.p[1], part);
                     acc[i][j] += xty_mfma16(xp[i].p[0], yp.p[0], part);
                 } else {
-                    acc[i][j] += xty_product(xp[i], yp.p[0]);
+                    acc[i][j] += xty_product(xp[i], yp.p[0], xty_zero());
                 }
                 xty_done(acc[i][j]);
             }
