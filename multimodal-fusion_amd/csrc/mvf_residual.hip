@@ -13,9 +13,10 @@
 // the squared differences: no cancellation): 4 to 64 lanes up to 1024 float32 or 1536 16-bit channels
 // (sums by lane exchanges only), a whole workgroup up to 4096.  A lane keeps its channels for the
 // whole launch, reads their weights from LDS, and has its next row under way while it works on one.
-// 262144 x 512 bfloat16 forward 232 us (4.6 TB/s), 500000 x 64 float32 forward and backward 104 + 153 us
-// (4.6 TB/s); 40007 x 1000 bfloat16 109 + 205 us (2.6 TB/s): there the backward keeps 64 column sums a
-// lane, two waves per SIMD, and vector work takes half its time.
+// 262144 x 512 bfloat16 forward 240 to 256 us by box (4.2 to 4.5 TB/s), 500000 x 64 float32 forward and backward
+// 262 to 268 us (109 + 157 + 9 in the kernel trace; 4.5 TB/s); 40007 x 1000 bfloat16 322 us (111 + 208 + 8; 2.5
+// TB/s): there a lane has 16 channels and the backward 64 column sums for them, with the rest more registers than
+// two waves per SIMD have, and one wave waits for its memory and works in turn.
 //
 // Backward, with n, o the normalised f and out, d the whole gradient of out and mean over channels:
 //   d  = d_out + r_out * (dh w_pre - o mean(dh w_pre o) - [layer] mean(dh w_pre))     = d_x
@@ -54,11 +55,12 @@ template <int TPR> struct RnBlock {
     static constexpr int THREADS = RN_THREADS;
     static constexpr int TEAMS = THREADS / TPR;
 };
-// Waves per SIMD a kernel with n channels a lane is compiled for: as many as its registers allow
-// without spills (the kernels for rows that are not aligned need a few more).  A launch fills the chip
-// with exactly that many: a second, partly filled round of workgroups costs as much as a whole one
-// (262144 x 512 bfloat16 forward 301 us with 768 workgroups of a kernel that fits 768, 387 us with 1024).
-// Backward 500000 x 64 float32 at 3, 4, 5 waves: 205, 200, 370 us (spills).
+// Waves per SIMD a kernel with n channels a lane is compiled for: as many as its registers allow with few
+// spills (float32 backward with one piece a lane up to 10 registers, with three 14 to 24; forward of unaligned
+// rows with one piece 2; the others none).  A launch fills the chip with exactly that many: a second, partly
+// filled round of workgroups costs as much as a whole one (262144 x 512 bfloat16 forward 245 to 256 us with
+// the 1024 workgroups that its kernel fits, 318 with 1280).  Forward and backward of 500000 x 64 float32 with 3, 4, 5
+// waves for the backward: 268, 268, 445 us (spills); of 40007 x 1000 bfloat16 with 1, 2: 326, 444 us (spills).
 static constexpr int rn_waves_fwd(int n) { return n <= 4 ? 6 : n <= 8 ? 4 : n <= 12 ? 3 : 2; }
 static constexpr int rn_waves_bwd(int n) { return n <= 4 ? 4 : n <= 12 ? 2 : 1; }
 
