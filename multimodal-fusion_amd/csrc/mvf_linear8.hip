@@ -19,8 +19,8 @@
 // matrix cores with exact parts (mvf_bf16x3.h): the tile's g column by column out of LDS, cut into three
 // parts; a value read back from 8 bits is one bf16.
 //
-// 2 M rows of 64 -> 64 columns: a Linear forward and backward 496 to 511 us by box (4.6 TB/s; as separate launches
-// of product, packing, grad_x and grad_W 671 us); behind BatchNorm 832 to 836 us.  A kernel trace, in which every
+// 2 M rows of 64 -> 64 columns: a Linear forward and backward 496 to 515 us by box (4.6 TB/s; as separate launches
+// of product, packing, grad_x and grad_W 671 us); behind BatchNorm 832 to 870 us.  A kernel trace, in which every
 // launch is slower, splits the latter into 93 us of statistics, 370 forward, 215 for the sums' pass, 246 for grad_z
 // and 23 for three folds.  Not bound by memory alone: the Linear's forward takes 286 us in the trace, 268 without its
 // packing, 261 without storing y and 220 without its products.  Two waves per SIMD leave matrix and vector work, and
